@@ -25,6 +25,7 @@ EXPORTS = [
     "gorch_cuda_topk_dev", "gorch_cuda_multinomial_dev",
     "gorch_cuda_lm_head_logits_dev", "gorch_cuda_lm_head_status", "gorch_cuda_lm_head_sample_dev",
     "gorch_cuda_generate_control_dev", "gorch_cuda_generate_step_dev",
+    "gorch_cuda_adjust_logits_dev", "gorch_cuda_generate_step_adjusted_dev",
     "gorch_cuda_softmax_dev", "gorch_cuda_cross_entropy_fwd_dev", "gorch_cuda_cross_entropy_bwd_dev",
 ]
 
@@ -39,6 +40,15 @@ class GenControl(C.Structure):
         ("cache_len", C.c_void_p), ("done", C.c_void_p), ("next_input", C.c_void_p), ("window_start", C.c_void_p),
         ("live_count", C.c_void_p), ("stop_tokens", C.c_int32 * GEN_MAX_STOPS), ("n_stop", C.c_int32),
         ("max_new", C.c_int32), ("max_seq", C.c_int32), ("cached", C.c_int32),
+    ]
+
+
+class LogitAdjust(C.Structure):
+    """GorchLogitAdjust of include/gorch_cuda_shim.h (device pointers)."""
+    _fields_ = [
+        ("penalties", C.c_void_p), ("history", C.c_void_p), ("history_stride", C.c_int64), ("history_lengths", C.c_void_p),
+        ("prompt_lengths", C.c_void_p), ("bias_offsets", C.c_void_p), ("bias_ids", C.c_void_p), ("bias_values", C.c_void_p),
+        ("n_bias", C.c_int64), ("mask", C.c_void_p), ("mask_stride", C.c_int64), ("n_masks", C.c_int64), ("mask_rows", C.c_void_p),
     ]
 
 
@@ -107,6 +117,8 @@ def load() -> C.CDLL:
         "gorch_cuda_cross_entropy_bwd_dev": (i32, [p, p, i32, i64, i64, i64, p, p, f32, p, i64, err]),
         "gorch_cuda_generate_control_dev": (i32, [p, p, p, C.POINTER(GenControl), i64, err]),
         "gorch_cuda_generate_step_dev": (i32, [p, p, i32, i64, i64, i64, p, p, p, p, C.POINTER(GenControl), err]),
+        "gorch_cuda_adjust_logits_dev": (i32, [p, p, i32, i64, i64, i64, C.POINTER(LogitAdjust), p, i64, err]),
+        "gorch_cuda_generate_step_adjusted_dev": (i32, [p, p, i32, i64, i64, i64, C.POINTER(LogitAdjust), p, p, p, p, C.POINTER(GenControl), err]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(L, name)

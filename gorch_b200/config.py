@@ -20,6 +20,11 @@ CFG_DTYPE = np.dtype(
     [("temperature", "<f4"), ("top_k", "<i4"), ("top_p", "<f4"), ("topp_mode", "<i4")]
 )
 
+# Per-row penalties, 16 bytes (GorchPenalty): repetition 1, presence 0 and frequency 0 are off.
+PENALTY_DTYPE = np.dtype(
+    [("repetition", "<f4"), ("presence", "<f4"), ("frequency", "<f4"), ("reserved", "<f4")]
+)
+
 # out_flags bits written per row by the sampling kernels.
 FLAG_BOUNDARY = 1 << 0      # uniform within 1e-6 of an edge of the chosen CDF interval
 FLAG_FALLBACK = 1 << 1      # walk fell through: id = V-1 (model/generate.go:239)

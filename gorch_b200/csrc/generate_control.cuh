@@ -34,7 +34,7 @@ constexpr int GC_LIVE = 0;
 constexpr int GC_STOP = 1;       // a stop token was sampled
 constexpr int GC_MAX_NEW = 2;    // MaxNewTokens tokens appended
 constexpr int GC_MAX_SEQ = 3;    // cached loops: the cache reached MaxSeq
-constexpr int GC_ERROR = 4;      // the sampler reported an unusable id, or the token buffer is full
+constexpr int GC_ERROR = 4;      // the sampler reported an unusable id or one that the row's mask does not allow, or the token buffer is full
 
 struct GenControlArgs {
   const int32_t* ids;        // [B] this step's sampled ids
@@ -54,6 +54,10 @@ struct GenControlArgs {
   int max_seq;
   int cached;
   uint32_t bad_flags;        // sampler flags that make an id unusable
+  const uint32_t* mask;      // [n_masks, mask_stride] words of allowed tokens, or null
+  long long mask_stride;
+  int n_masks;
+  const int32_t* mask_rows;  // [B] or null: row b has mask b
   int B;
 };
 
@@ -72,6 +76,10 @@ __global__ void __launch_bounds__(GC_NT) generate_control_kernel(const __grid_co
     if (done != GC_LIVE) continue;
     if (n >= A.max_new) { A.done[b] = GC_MAX_NEW; continue; }
     if (id < 0 || (fl & A.bad_flags) != 0u) { A.done[b] = GC_ERROR; continue; }
+    if (A.mask != nullptr) {
+      const int m = A.mask_rows ? A.mask_rows[b] : b;
+      if (m >= 0 && m < A.n_masks && !((A.mask[m * A.mask_stride + (id >> 5)] >> (id & 31)) & 1u)) { A.done[b] = GC_ERROR; continue; }
+    }
     bool stop = false;
     for (int s = 0; s < A.n_stop; s++) stop |= (id == A.stops[s]);
     if (stop) { A.done[b] = GC_STOP; continue; }

@@ -31,6 +31,7 @@
 #include "topk_large.cuh"
 #include "generate_control.cuh"
 #include "row_softmax.cuh"
+#include "adjust_logits.cuh"
 #include "lm_head.cuh"
 
 namespace {
@@ -738,6 +739,15 @@ cudaError_t topk_large_attributes() {
   return e != cudaSuccess ? e : cudaFuncSetAttribute(gs::topk_large_kernel<uint16_t, SH>, cudaFuncAttributeMaxDynamicSharedMemorySize, SH::DYN_BYTES);
 }
 
+cudaError_t adjust_attributes() {
+  const int f = gs::adjust_words_bytes(true), h = gs::adjust_words_bytes(false);
+  cudaError_t e = cudaFuncSetAttribute(gs::adjust_logits_kernel<float, true, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, f);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(gs::adjust_logits_kernel<float, false, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, f);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(gs::adjust_logits_kernel<uint16_t, true, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, h);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(gs::adjust_logits_kernel<uint16_t, false, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, h);
+  return e;
+}
+
 }  // namespace
 
 extern "C" {
@@ -833,6 +843,7 @@ GorchCudaCtxRef gorch_cuda_create_ctx(int device, char** errOut) {
   if ((e = cudaFuncSetAttribute(gs::row_softmax_kernel<uint16_t>, cudaFuncAttributeMaxDynamicSharedMemorySize, gs::RS_DYN_BYTES)) != cudaSuccess) return fail("cudaFuncSetAttribute", e);
   if ((e = cudaFuncSetAttribute(gs::row_softmax_resident_kernel<float>, cudaFuncAttributeMaxDynamicSharedMemorySize, gs::RR_SLICE)) != cudaSuccess) return fail("cudaFuncSetAttribute", e);
   if ((e = cudaFuncSetAttribute(gs::row_softmax_resident_kernel<uint16_t>, cudaFuncAttributeMaxDynamicSharedMemorySize, gs::RR_SLICE)) != cudaSuccess) return fail("cudaFuncSetAttribute", e);
+  if ((e = adjust_attributes()) != cudaSuccess) return fail("cudaFuncSetAttribute", e);
   if ((e = cudaFuncSetAttribute(gs::w256::wide_rows_kernel<uint16_t>, cudaFuncAttributeMaxDynamicSharedMemorySize, gs::w256::W_DYN_BYTES)) != cudaSuccess) return fail("cudaFuncSetAttribute", e);
   return c;
 }
@@ -1403,8 +1414,7 @@ int gorch_cuda_multinomial_dev(GorchCudaCtxRef ctx, const float* probs, int64_t 
   return GORCH_CUDA_OK;
 }
 
-static int launch_generate_control(Ctx* c, const int32_t* ids, const uint32_t* flags,
-                                   const GorchGenControl* gc, int64_t B, char** errOut) {
+static int check_generate_control(const int32_t* ids, const GorchGenControl* gc, int64_t B, char** errOut) {
   static_assert(GORCH_GEN_MAX_STOPS == gs::GC_MAX_STOPS && GORCH_GEN_STOP == gs::GC_STOP &&
                 GORCH_GEN_MAX_NEW == gs::GC_MAX_NEW && GORCH_GEN_MAX_SEQ == gs::GC_MAX_SEQ &&
                 GORCH_GEN_ERROR == gs::GC_ERROR, "generate-control codes");
@@ -1421,7 +1431,14 @@ static int launch_generate_control(Ctx* c, const int32_t* ids, const uint32_t* f
     set_err(errOut, "gorch_cuda: null pointer in the generate-control record");
     return GORCH_CUDA_ERR_BAD_ARG;
   }
-  gs::GenControlArgs a;
+  return GORCH_CUDA_OK;
+}
+
+static int launch_generate_control(Ctx* c, const int32_t* ids, const uint32_t* flags,
+                                   const GorchGenControl* gc, int64_t B, char** errOut, const GorchLogitAdjust* adj = nullptr) {
+  const int rc = check_generate_control(ids, gc, B, errOut);
+  if (rc || B == 0) return rc;
+  gs::GenControlArgs a{};
   a.ids = ids; a.flags = flags;
   a.tokens = gc->tokens; a.capacity = gc->capacity; a.lengths = gc->lengths; a.n_new = gc->n_new;
   a.cache_len = gc->cache_len; a.done = gc->done; a.next_input = gc->next_input;
@@ -1430,6 +1447,9 @@ static int launch_generate_control(Ctx* c, const int32_t* ids, const uint32_t* f
   a.n_stop = gc->n_stop; a.max_new = gc->max_new; a.max_seq = gc->max_seq; a.cached = gc->cached ? 1 : 0;
   a.bad_flags = GORCH_FLAG_INTERNAL | GORCH_FLAG_BAD_CFG;
   a.B = static_cast<int>(B);
+  if (adj && adj->mask) {                                    // (ids are below V, which the mask covers)
+    a.mask = adj->mask; a.mask_stride = adj->mask_stride; a.n_masks = static_cast<int>(adj->n_masks); a.mask_rows = adj->mask_rows;
+  }
   CUDA_TRY(launch(c, gs::generate_control_kernel, 1, gs::GC_NT, 0, true, a), errOut);
   c->counters.kernel_launches += 1;
   return GORCH_CUDA_OK;
@@ -1465,6 +1485,132 @@ int gorch_cuda_generate_step_dev(GorchCudaCtxRef ctx, const void* logits, int dt
     if (rc) return rc;
   }
   return launch_generate_control(c, out_ids, out_flags, gc, B, errOut);
+}
+
+// Whether two [B, stride] tensors of rows of V elements share an element. Rows of one stride may lie side by side.
+static bool rows_overlap(const void* a, int64_t sa, size_t ea, const void* b, int64_t sb, size_t eb, int64_t B, int64_t V) {
+  const uintptr_t a0 = reinterpret_cast<uintptr_t>(a), b0 = reinterpret_cast<uintptr_t>(b);
+  const uintptr_t a1 = a0 + (static_cast<uintptr_t>(B - 1) * sa + V) * ea, b1 = b0 + (static_cast<uintptr_t>(B - 1) * sb + V) * eb;
+  if (a0 >= b1 || b0 >= a1) return false;
+  const uintptr_t pitch = static_cast<uintptr_t>(sa) * ea;
+  if (pitch != static_cast<uintptr_t>(sb) * eb) return true;
+  const uintptr_t d = a0 > b0 ? (a0 - b0) % pitch : (pitch - (b0 - a0) % pitch) % pitch;   // where a's rows start within b's pitch
+  return d < static_cast<uintptr_t>(V) * eb || pitch - d < static_cast<uintptr_t>(V) * ea;
+}
+
+static int check_adjust(const GorchLogitAdjust* adj, int64_t B, int64_t V, bool own_history, char** errOut) {
+  if (!adj) { set_err(errOut, "gorch_cuda: null logit-adjust record"); return GORCH_CUDA_ERR_BAD_ARG; }
+  if (B == 0) return GORCH_CUDA_OK;
+  auto off4 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) != 0; };
+  if (off4(adj->penalties) || off4(adj->bias_offsets) || off4(adj->bias_ids) || off4(adj->bias_values) || off4(adj->mask) || off4(adj->mask_rows) ||
+      (own_history && adj->penalties && (off4(adj->history) || off4(adj->history_lengths) || off4(adj->prompt_lengths)))) {
+    set_err(errOut, "gorch_cuda: pointer of the logit-adjust record not aligned to its element type");
+    return GORCH_CUDA_ERR_BAD_ARG;
+  }
+  if (adj->penalties && own_history) {
+    if (!adj->history_lengths || (!adj->history && adj->history_stride > 0)) {
+      set_err(errOut, "gorch_cuda: penalties need a history and its lengths");
+      return GORCH_CUDA_ERR_BAD_ARG;
+    }
+    if (adj->history_stride < 0) { set_err(errOut, "gorch_cuda: negative history_stride"); return GORCH_CUDA_ERR_BAD_ARG; }
+    if (adj->history_stride >= (1ll << 30)) { set_err(errOut, "gorch_cuda: history_stride beyond 2^30 - 1"); return GORCH_CUDA_ERR_LIMIT; }
+  }
+  if (adj->bias_offsets) {
+    if (adj->n_bias < 0 || (adj->n_bias > 0 && (!adj->bias_ids || !adj->bias_values))) {
+      set_err(errOut, "gorch_cuda: biases need their ids and values, n_bias >= 0");
+      return GORCH_CUDA_ERR_BAD_ARG;
+    }
+    if (adj->n_bias > 0x7fffffffll) { set_err(errOut, "gorch_cuda: n_bias beyond 31 bits"); return GORCH_CUDA_ERR_LIMIT; }
+  }
+  if (adj->mask) {
+    if (adj->n_masks < 1 || adj->mask_stride < (V + 31) / 32 || (!adj->mask_rows && adj->n_masks < B)) {
+      set_err(errOut, "gorch_cuda: masks need n_masks >= 1 (one per row without mask_rows) and mask_stride >= (V + 31) / 32, got %lld and %lld",
+              (long long)adj->n_masks, (long long)adj->mask_stride);
+      return GORCH_CUDA_ERR_BAD_ARG;
+    }
+    if (adj->n_masks > 0x7fffffffll) { set_err(errOut, "gorch_cuda: n_masks beyond 31 bits"); return GORCH_CUDA_ERR_LIMIT; }
+  }
+  return GORCH_CUDA_OK;
+}
+
+// One launch of adjust_logits_kernel. gc: the rows' tokens and the rows to pass over come from there.
+static int launch_adjust(Ctx* c, const void* logits, int dtype, int64_t B, int64_t V, int64_t row_stride, const GorchLogitAdjust* adj,
+                         void* out, int64_t out_stride, const GorchGenControl* gc, char** errOut) {
+  gs::AdjustArgs a{};
+  a.x = logits; a.row_stride = row_stride; a.out = out; a.out_stride = out_stride;
+  a.V = static_cast<int32_t>(V);
+  if (adj->penalties) {
+    a.penalties = reinterpret_cast<const float*>(adj->penalties);
+    if (gc) { a.history = gc->tokens; a.history_stride = gc->capacity; a.lengths = gc->lengths; a.n_new = gc->n_new; }
+    else { a.history = adj->history; a.history_stride = adj->history_stride; a.lengths = adj->history_lengths; a.prompt_lengths = adj->prompt_lengths; }
+  }
+  if (adj->bias_offsets && adj->n_bias > 0) {
+    a.bias_offsets = adj->bias_offsets; a.bias_ids = adj->bias_ids; a.bias_values = adj->bias_values; a.n_bias = static_cast<int32_t>(adj->n_bias);
+  }
+  if (adj->mask) { a.mask = adj->mask; a.mask_stride = adj->mask_stride; a.n_masks = static_cast<int32_t>(adj->n_masks); a.mask_rows = adj->mask_rows; }
+  if (gc) a.row_done = gc->done;
+  const bool in_place = out == logits, words = a.penalties || a.bias_offsets;
+  if (in_place && !words && !a.mask) return GORCH_CUDA_OK;
+  const int64_t per = static_cast<int64_t>(gs::AL_NT) * gs::AL_U;
+  const int64_t nchunk = (row_vectors(V, dtype) + per - 1) / per;
+  if (B * nchunk > 0x7fffffffll) { set_err(errOut, "gorch_cuda: batch beyond the limit of a launch"); return GORCH_CUDA_ERR_LIMIT; }
+  a.nchunk = static_cast<int32_t>(nchunk);
+  const unsigned grid = static_cast<unsigned>(B * nchunk);
+  const size_t dyn = words ? static_cast<size_t>(gs::adjust_words_bytes(dtype == GORCH_CUDA_F32)) : 0;
+  auto pick = [&](auto type) {
+    typedef decltype(type) E;
+    auto* k = in_place ? (words ? gs::adjust_logits_kernel<E, true, true> : gs::adjust_logits_kernel<E, true, false>)
+                       : (words ? gs::adjust_logits_kernel<E, false, true> : gs::adjust_logits_kernel<E, false, false>);
+    return launch(c, k, grid, gs::AL_NT, dyn, true, a);
+  };
+  CUDA_TRY(dtype == GORCH_CUDA_F32 ? pick(float()) : pick(uint16_t()), errOut);
+  c->counters.kernel_launches += 1;
+  return GORCH_CUDA_OK;
+}
+
+int gorch_cuda_adjust_logits_dev(GorchCudaCtxRef ctx, const void* logits, int dtype, int64_t B, int64_t V, int64_t row_stride,
+                                 const GorchLogitAdjust* adjust, void* out, int64_t out_stride, char** errOut) {
+  Ctx* c = static_cast<Ctx*>(ctx);
+  if (!c) { set_err(errOut, "gorch_cuda: null context"); return GORCH_CUDA_ERR_BAD_ARG; }
+  int rc = check_shape(dtype, B, V, row_stride, errOut);
+  if (rc || (rc = check_adjust(adjust, B, V, true, errOut))) return rc;
+  if (out_stride < V) { set_err(errOut, "gorch_cuda: out_stride %lld below V", (long long)out_stride); return GORCH_CUDA_ERR_BAD_ARG; }
+  if (B == 0) return GORCH_CUDA_OK;
+  if (!logits || !out) { set_err(errOut, "gorch_cuda: null pointer argument"); return GORCH_CUDA_ERR_BAD_ARG; }
+  const size_t es = elem_size(dtype);
+  if ((reinterpret_cast<uintptr_t>(logits) % es) != 0 || (reinterpret_cast<uintptr_t>(out) % es) != 0) {
+    set_err(errOut, "gorch_cuda: pointer not aligned to its element type");
+    return GORCH_CUDA_ERR_BAD_ARG;
+  }
+  const bool in_place = out == logits && (out_stride == row_stride || B == 1);
+  if (!in_place && rows_overlap(logits, row_stride, es, out, out_stride, es, B, V)) {
+    set_err(errOut, "gorch_cuda: out overlaps the logits without being the same rows");
+    return GORCH_CUDA_ERR_BAD_ARG;
+  }
+  CUDA_TRY(cudaSetDevice(c->device), errOut);
+  return launch_adjust(c, logits, dtype, B, V, row_stride, adjust, out, out_stride, nullptr, errOut);
+}
+
+int gorch_cuda_generate_step_adjusted_dev(GorchCudaCtxRef ctx, void* logits, int dtype, int64_t B, int64_t V, int64_t row_stride,
+                                          const GorchLogitAdjust* adjust, const GorchSampleCfg* cfgs, const double* uniforms,
+                                          int32_t* out_ids, uint32_t* out_flags, const GorchGenControl* gc, char** errOut) {
+  Ctx* c = static_cast<Ctx*>(ctx);
+  if (!c) { set_err(errOut, "gorch_cuda: null context"); return GORCH_CUDA_ERR_BAD_ARG; }
+  int rc = check_shape(dtype, B, V, row_stride, errOut);
+  // (the records are looked at before anything is launched: a refused step has not touched the logits)
+  if (rc || (rc = check_adjust(adjust, B, V, false, errOut)) || (rc = check_generate_control(out_ids, gc, B, errOut))) return rc;
+  if (B == 0) return GORCH_CUDA_OK;
+  if (!logits || !cfgs || !uniforms) { set_err(errOut, "gorch_cuda: null pointer argument"); return GORCH_CUDA_ERR_BAD_ARG; }
+  if ((reinterpret_cast<uintptr_t>(logits) % elem_size(dtype)) != 0) {
+    set_err(errOut, "gorch_cuda: logits pointer not aligned to its element size");
+    return GORCH_CUDA_ERR_BAD_ARG;
+  }
+  if (adjust->penalties && gc->capacity >= (1ll << 30)) { set_err(errOut, "gorch_cuda: capacity beyond 2^30 - 1 tokens"); return GORCH_CUDA_ERR_LIMIT; }
+  CUDA_TRY(cudaSetDevice(c->device), errOut);
+  if ((rc = launch_adjust(c, logits, dtype, B, V, row_stride, adjust, logits, row_stride, gc, errOut))) return rc;
+  rc = launch_rows(c, logits, dtype, B, V, row_stride, cfgs, uniforms, out_ids, out_flags, nullptr, nullptr, 0, errOut, nullptr, gc->done);
+  if (rc) return rc;
+  return launch_generate_control(c, out_ids, out_flags, gc, B, errOut, adjust);
 }
 
 // CTAs per row of the resident softmax: as few as leave room for two slices per SM (any number up to eight), twice as many

@@ -117,9 +117,17 @@ class DeviceGenerateState:
         rc = self.s._lib.gorch_cuda_generate_control_dev(self.s._ctx, ids_ptr, flags_ptr, C.byref(self.gc), self.B, C.byref(err))
         _check(self.s._lib, rc, err)
 
-    def step(self, logits_ptr: int, dtype: int, V: int, row_stride: int, cfgs_ptr: int, uniforms_ptr: int) -> None:
-        """Sample every row of logits [B,V] and apply one loop iteration; asynchronous."""
+    def step(self, logits_ptr: int, dtype: int, V: int, row_stride: int, cfgs_ptr: int, uniforms_ptr: int, rules=None) -> None:
+        """Sample every row of logits [B,V] and apply one loop iteration; asynchronous. rules (a rules.LogitRules or a
+        _lib.LogitAdjust record): the live rows' logits are adjusted by them first, in place, with the tokens of this state as
+        their history (gorch_cuda_generate_step_adjusted_dev)."""
         err = C.c_void_p()
+        if rules is not None:
+            rc = self.s._lib.gorch_cuda_generate_step_adjusted_dev(
+                self.s._ctx, logits_ptr, dtype, self.B, V, row_stride, C.byref(getattr(rules, "record", rules)), cfgs_ptr,
+                uniforms_ptr, self.ids_ptr, self.flags_ptr, C.byref(self.gc), C.byref(err))
+            _check(self.s._lib, rc, err)
+            return
         rc = self.s._lib.gorch_cuda_generate_step_dev(self.s._ctx, logits_ptr, dtype, self.B, V, row_stride, cfgs_ptr,
                                                       uniforms_ptr, self.ids_ptr, self.flags_ptr, C.byref(self.gc), C.byref(err))
         _check(self.s._lib, rc, err)
@@ -152,12 +160,15 @@ class DeviceGenerateState:
 
 
 def generate_on_device(model, prompts, cfgs, uniforms, sampler: CudaSampler, max_new: int, max_seq: int,
-                       stop_tokens=(), loop: int = LOOP_CACHED, poll_every: int = 8) -> dict:
+                       stop_tokens=(), loop: int = LOOP_CACHED, poll_every: int = 8, rules=None) -> dict:
     """Runs B sequences to completion. `cfgs` is a CFG_DTYPE array [B] (each row's sampling
     fields), `uniforms` a float64 array [max_new, B]: row b consumes uniforms[i, b] in its i-th
     iteration, as the reference draws one value per sampled token. `model.prefill_dev(state)` and
     `model.forward_dev(state)` each return (logits_ptr, dtype, V, row_stride) for logits [B,V]
-    on the device. Returns DeviceGenerateState.results()."""
+    on the device. `rules` (rules.LogitRules of the B rows): penalties over each row's own tokens, biases and
+    masks, applied to every step's logits where they lie (see DeviceGenerateState.step); `rules` may also be a
+    function of the step's number that returns them, for grammars whose masks change as tokens are added.
+    Returns DeviceGenerateState.results()."""
     cfgs = np.ascontiguousarray(cfgs, dtype=CFG_DTYPE)
     uniforms = np.ascontiguousarray(uniforms, dtype=np.float64).reshape(max(int(max_new), 0), -1)
     st = DeviceGenerateState(sampler, prompts, max_new, max_seq, stop_tokens, loop)
@@ -176,7 +187,7 @@ def generate_on_device(model, prompts, cfgs, uniforms, sampler: CudaSampler, max
         if st.B and max_new > 0:
             logits_ptr, dtype, V, stride = model.prefill_dev(st)
             for i in range(max_new):
-                st.step(logits_ptr, dtype, V, stride, p_cfg, p_uni + 8 * st.B * i)
+                st.step(logits_ptr, dtype, V, stride, p_cfg, p_uni + 8 * st.B * i, rules(i) if callable(rules) else rules)
                 steps += 1
                 if i + 1 == max_new:
                     break

@@ -392,6 +392,16 @@ class CudaSampler:
                 self._lib.gorch_cuda_buffer_free(b)
         return ids, flags
 
+    # ---- a request's rules in front of the sampling step
+    def adjust_logits_ptrs(self, logits_ptr: int, dtype: int, B: int, V: int, row_stride: int, adjust, out_ptr: int,
+                           out_stride: int) -> None:
+        """gorch_cuda_adjust_logits_dev: penalties, biases and masks of `adjust` (a _lib.LogitAdjust record of device
+        pointers) on logits [B, V]; out_ptr may be logits_ptr. Device pointers, asynchronous."""
+        err = C.c_void_p()
+        rc = self._lib.gorch_cuda_adjust_logits_dev(self._ctx, logits_ptr, dtype, B, V, row_stride,
+                                                    C.byref(adjust) if adjust is not None else None, out_ptr, out_stride, C.byref(err))
+        _check(self._lib, rc, err)
+
     # ---- the LM-head projection in front of the sampling step (model/qwen/qwen.go:80-85)
     def lm_head_logits_ptrs(self, x_ptr: int, ldx: int, w_ptr: int, ldw: int, B: int, V: int, K: int,
                             out_ptr: int, ld_out: int) -> None:

@@ -333,6 +333,56 @@ int gorch_cuda_generate_step_dev(GorchCudaCtxRef ctx, const void* logits, int dt
                                  const double* uniforms, int32_t* out_ids, uint32_t* out_flags,
                                  const GorchGenControl* gc, char** errOut);
 
+/* The rules of a request on its logits, in front of the sampling step (no counterpart in the reference, which
+ * samples from the bare logits, model/generate.go:75-79). For row b and token v, in f32, every operation
+ * rounded once and the result once more to bf16 for bf16 logits:
+ *   c = how often v is among the row's generated tokens; held = v is in its prompt or among them
+ *   y = held ? (x > 0 ? x / repetition : x * repetition) : x
+ *   y = c > 0 ? (y - frequency * c) - presence : y
+ *   y = y + bias       of the entry listed for v, of the last one if there are several
+ *   y = -Inf           where the row's mask has a 0 for v, whatever x held (NaN and infinities too)
+ * A logit that no rule touches keeps its bits. A row whose mask allows nothing comes out as -Inf
+ * throughout, and the sampling calls treat it as any such row (GORCH_FLAG_NONFINITE; temperature 0:
+ * token 0). All pointers are device pointers owned by the caller; a part whose first pointer is NULL
+ * is off. Token ids outside [0, V) in a history or a bias map are passed over. */
+typedef struct {
+  float repetition; /* 1: off; otherwise above 0 */
+  float presence;   /* 0: off */
+  float frequency;  /* 0: off */
+  float reserved;
+} GorchPenalty;
+typedef struct {
+  const GorchPenalty* penalties; /* [B], or NULL: no penalties, and the four below are not looked at */
+  const int32_t* history;        /* [B, history_stride] token ids, prompt first */
+  int64_t history_stride;        /* at most 2^30 - 1 */
+  const int32_t* history_lengths; /* [B] tokens that a row holds: 0 .. history_stride (others are taken as the nearer end) */
+  const int32_t* prompt_lengths; /* [B] how many of them are prompt, or NULL: none */
+  const int32_t* bias_offsets;   /* [B + 1] row b has the entries bias_offsets[b] .. bias_offsets[b + 1] - 1; or NULL: no biases */
+  const int32_t* bias_ids;       /* [n_bias] */
+  const float* bias_values;      /* [n_bias] */
+  int64_t n_bias;                /* entries in all; offsets beyond it are taken as n_bias */
+  const uint32_t* mask;          /* [n_masks, mask_stride] words, bit v % 32 of word v / 32: token v is allowed; or NULL: no masks */
+  int64_t mask_stride;           /* words from one mask to the next, at least (V + 31) / 32 */
+  int64_t n_masks;
+  const int32_t* mask_rows;      /* [B] the row's mask, outside [0, n_masks): none; or NULL: row b has mask b */
+} GorchLogitAdjust;
+/* out [B,out_stride] has the logits' type; it may be `logits` itself with the same stride (in place:
+ * then only what changes is read and written), and must not overlap them otherwise. Device pointers,
+ * asynchronous on the context's stream, no memory of the context's is used. */
+int gorch_cuda_adjust_logits_dev(GorchCudaCtxRef ctx, const void* logits, int dtype, int64_t B,
+                                 int64_t V, int64_t row_stride, const GorchLogitAdjust* adjust,
+                                 void* out, int64_t out_stride, char** errOut);
+/* gorch_cuda_generate_step_dev behind the rules: the logits of the live rows are adjusted in place, then
+ * sampled, then the control step runs. The row's tokens are taken from the control record (gc->tokens,
+ * gc->lengths; the last gc->n_new of them are the generated ones), and adjust's history fields are not
+ * looked at. A sampled token that the row's mask does not allow (what the sampling calls return where the
+ * mask leaves nothing) ends the row with GORCH_GEN_ERROR, nothing appended. */
+int gorch_cuda_generate_step_adjusted_dev(GorchCudaCtxRef ctx, void* logits, int dtype, int64_t B,
+                                          int64_t V, int64_t row_stride, const GorchLogitAdjust* adjust,
+                                          const GorchSampleCfg* cfgs, const double* uniforms,
+                                          int32_t* out_ids, uint32_t* out_flags,
+                                          const GorchGenControl* gc, char** errOut);
+
 /* Row softmax, log-softmax and cross-entropy over x [B,V] (f32, or bf16 upcast) at vocabulary
  * scale, as device ops (device pointers, asynchronous on the context's stream).
  * gorch_cuda_softmax_dev: log_softmax == 0: gorch.Softmax (ops.go:527-563), out = exp(x - max) /
