@@ -27,6 +27,7 @@ EXPORTS = [
     "gorch_cuda_generate_control_dev", "gorch_cuda_generate_step_dev",
     "gorch_cuda_adjust_logits_dev", "gorch_cuda_generate_step_adjusted_dev",
     "gorch_cuda_softmax_dev", "gorch_cuda_cross_entropy_fwd_dev", "gorch_cuda_cross_entropy_bwd_dev",
+    "gorch_cuda_distill_fwd_dev", "gorch_cuda_distill_bwd_dev",
 ]
 
 
@@ -115,6 +116,8 @@ def load() -> C.CDLL:
         "gorch_cuda_softmax_dev": (i32, [p, p, i32, i64, i64, i64, p, i64, i32, err]),
         "gorch_cuda_cross_entropy_fwd_dev": (i32, [p, p, i32, i64, i64, i64, p, p, p, p, err]),
         "gorch_cuda_cross_entropy_bwd_dev": (i32, [p, p, i32, i64, i64, i64, p, p, f32, p, i64, err]),
+        "gorch_cuda_distill_fwd_dev": (i32, [p, p, i32, i64, i64, i64, p, p, i64, i64, f32, p, p, p, err]),
+        "gorch_cuda_distill_bwd_dev": (i32, [p, p, i32, i64, i64, i64, p, p, i64, i64, f32, p, p, f32, i32, p, i64, err]),
         "gorch_cuda_generate_control_dev": (i32, [p, p, p, C.POINTER(GenControl), i64, err]),
         "gorch_cuda_generate_step_dev": (i32, [p, p, i32, i64, i64, i64, p, p, p, p, C.POINTER(GenControl), err]),
         "gorch_cuda_adjust_logits_dev": (i32, [p, p, i32, i64, i64, i64, C.POINTER(LogitAdjust), p, i64, err]),

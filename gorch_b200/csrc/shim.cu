@@ -32,6 +32,7 @@
 #include "generate_control.cuh"
 #include "row_softmax.cuh"
 #include "adjust_logits.cuh"
+#include "distill.cuh"
 #include "lm_head.cuh"
 
 namespace {
@@ -1769,6 +1770,86 @@ int gorch_cuda_cross_entropy_bwd_dev(GorchCudaCtxRef ctx, const void* logits, in
   a.mode = gs::RS_CE_BWD; a.targets = targets; a.row_lse = const_cast<float*>(row_lse);
   a.scale = scale; a.out = dx; a.out_stride = dx_stride;
   return launch_row_softmax(c, dtype, a, errOut);
+}
+
+static int distill_args(Ctx* c, gs::DistillArgs& a, const void* logits, int dtype, int64_t B, int64_t V, int64_t row_stride,
+                        const int32_t* ids, const float* teacher, int64_t k, int64_t t_stride, float T, char** errOut) {
+  if (!c) { set_err(errOut, "gorch_cuda: null context"); return GORCH_CUDA_ERR_BAD_ARG; }
+  const int rc = check_shape(dtype, B, V, row_stride, errOut);
+  if (rc) return rc;
+  if (k < 1 || t_stride < k) { set_err(errOut, "gorch_cuda: distillation needs k >= 1 and teacher_stride >= k, got %lld and %lld", (long long)k, (long long)t_stride); return GORCH_CUDA_ERR_BAD_ARG; }
+  if (k > 16384) { set_err(errOut, "gorch_cuda: k %lld beyond 16384", (long long)k); return GORCH_CUDA_ERR_LIMIT; }
+  if (!(T >= gs::DS_MIN_T) || !(T <= gs::DS_MAX_T)) { set_err(errOut, "gorch_cuda: temperature %g outside 1e-6 .. 1e6", static_cast<double>(T)); return GORCH_CUDA_ERR_BAD_ARG; }
+  if (B == 0) return GORCH_CUDA_OK;
+  if (!logits || !ids || !teacher) { set_err(errOut, "gorch_cuda: null pointer argument"); return GORCH_CUDA_ERR_BAD_ARG; }
+  if ((reinterpret_cast<uintptr_t>(logits) % elem_size(dtype)) != 0 || (reinterpret_cast<uintptr_t>(ids) & 3u) || (reinterpret_cast<uintptr_t>(teacher) & 3u)) {
+    set_err(errOut, "gorch_cuda: pointer not aligned to its element type");
+    return GORCH_CUDA_ERR_BAD_ARG;
+  }
+  a.x = logits; a.row_stride = row_stride; a.V = static_cast<int32_t>(V); a.B = B;
+  a.ids = ids; a.teacher = teacher; a.k = static_cast<int32_t>(k); a.t_stride = t_stride;
+  a.T = T; a.sc = gs::ds_scale(T);
+  return GORCH_CUDA_OK;
+}
+
+int gorch_cuda_distill_fwd_dev(GorchCudaCtxRef ctx, const void* logits, int dtype, int64_t B, int64_t V, int64_t row_stride,
+                               const int32_t* teacher_ids, const float* teacher_logits, int64_t k, int64_t teacher_stride,
+                               float temperature, float* row_loss, float* row_stats, float* mean_loss, char** errOut) {
+  Ctx* c = static_cast<Ctx*>(ctx);
+  gs::DistillArgs a{};
+  const int rc = distill_args(c, a, logits, dtype, B, V, row_stride, teacher_ids, teacher_logits, k, teacher_stride, temperature, errOut);
+  if (rc || B == 0) return rc;
+  if (!row_loss || !row_stats) { set_err(errOut, "gorch_cuda: null pointer argument"); return GORCH_CUDA_ERR_BAD_ARG; }
+  if ((reinterpret_cast<uintptr_t>(row_loss) & 3u) || (reinterpret_cast<uintptr_t>(row_stats) & 3u) || (reinterpret_cast<uintptr_t>(mean_loss) & 3u)) {
+    set_err(errOut, "gorch_cuda: pointer not aligned to its element type");
+    return GORCH_CUDA_ERR_BAD_ARG;
+  }
+  a.row_loss = row_loss; a.stats = row_stats;
+  CUDA_TRY(cudaSetDevice(c->device), errOut);
+  const int64_t nvec = row_vectors(V, dtype);
+  int C = 1;
+  while (C < gs::DF_MAX_C && B * C < 8ll * c->sm_count && nvec / (2 * C) >= gs::DF_NT) C *= 2;
+  if (B * C > 0x7fffffffll) { set_err(errOut, "gorch_cuda: batch beyond the limit of a launch"); return GORCH_CUDA_ERR_LIMIT; }
+  auto* kernel = dtype == GORCH_CUDA_F32 ? gs::distill_fwd_kernel<float> : gs::distill_fwd_kernel<uint16_t>;
+  CUDA_TRY(launch_clusters(c, kernel, static_cast<unsigned>(B * C), gs::DF_NT, 0, true, C, a), errOut);
+  c->counters.kernel_launches += 1;
+  if (mean_loss) {
+    CUDA_TRY(launch(c, gs::mean_loss_kernel, 1, 256, 0, true, static_cast<const float*>(row_loss), B, mean_loss), errOut);
+    c->counters.kernel_launches += 1;
+  }
+  return GORCH_CUDA_OK;
+}
+
+int gorch_cuda_distill_bwd_dev(GorchCudaCtxRef ctx, const void* logits, int dtype, int64_t B, int64_t V, int64_t row_stride,
+                               const int32_t* teacher_ids, const float* teacher_logits, int64_t k, int64_t teacher_stride,
+                               float temperature, const float* row_stats, const float* row_grads, float scale, int accumulate,
+                               float* dx, int64_t dx_stride, char** errOut) {
+  Ctx* c = static_cast<Ctx*>(ctx);
+  gs::DistillArgs a{};
+  const int rc = distill_args(c, a, logits, dtype, B, V, row_stride, teacher_ids, teacher_logits, k, teacher_stride, temperature, errOut);
+  if (rc) return rc;
+  if (dx_stride < V) { set_err(errOut, "gorch_cuda: dx_stride %lld below V", (long long)dx_stride); return GORCH_CUDA_ERR_BAD_ARG; }
+  if (B == 0) return GORCH_CUDA_OK;
+  if (!row_stats || !dx) { set_err(errOut, "gorch_cuda: null pointer argument"); return GORCH_CUDA_ERR_BAD_ARG; }
+  if ((reinterpret_cast<uintptr_t>(row_stats) & 3u) || (reinterpret_cast<uintptr_t>(row_grads) & 3u) || (reinterpret_cast<uintptr_t>(dx) & 3u)) {
+    set_err(errOut, "gorch_cuda: pointer not aligned to its element type");
+    return GORCH_CUDA_ERR_BAD_ARG;
+  }
+  const bool same = dtype == GORCH_CUDA_F32 && dx == logits && (dx_stride == row_stride || B == 1) && !accumulate;
+  if (!same && rows_overlap(logits, row_stride, elem_size(dtype), dx, dx_stride, 4, B, V)) {
+    set_err(errOut, "gorch_cuda: dx overlaps the logits without being the same rows");
+    return GORCH_CUDA_ERR_BAD_ARG;
+  }
+  a.stats = const_cast<float*>(row_stats); a.row_grads = row_grads; a.scale = scale; a.accumulate = accumulate ? 1 : 0;
+  a.dx = dx; a.dx_stride = dx_stride;
+  const int64_t per = static_cast<int64_t>(gs::DB_NT) * gs::DB_U, nchunk = (row_vectors(V, dtype) + per - 1) / per;
+  if (B * nchunk > 0x7fffffffll) { set_err(errOut, "gorch_cuda: batch beyond the limit of a launch"); return GORCH_CUDA_ERR_LIMIT; }
+  a.nchunk = static_cast<int32_t>(nchunk);
+  CUDA_TRY(cudaSetDevice(c->device), errOut);
+  auto* kernel = dtype == GORCH_CUDA_F32 ? gs::distill_bwd_kernel<float> : gs::distill_bwd_kernel<uint16_t>;
+  CUDA_TRY(launch(c, kernel, static_cast<unsigned>(B * nchunk), gs::DB_NT, 0, true, a), errOut);
+  c->counters.kernel_launches += 1;
+  return GORCH_CUDA_OK;
 }
 
 int64_t gorch_cuda_sample_row(GorchCudaCtxRef ctx, const float* logits, int64_t n,

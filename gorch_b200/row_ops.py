@@ -1,5 +1,6 @@
 """gorch.Softmax, gorch.LogSoftmax and gorch.CrossEntropyLoss (forward and backward) over [B, V]
-logits at vocabulary scale, on the device (ops.go:527-603, loss.go:55-141).
+logits at vocabulary scale, on the device (ops.go:527-603, loss.go:55-141); beside them the distillation
+loss against a teacher's top logits and its gradient.
 
 The `*_ptrs` functions take device pointers and are asynchronous on the context's stream; the
 array functions upload, run, and download (tests and small jobs). Without the CUDA library every
@@ -33,6 +34,27 @@ def cross_entropy_bwd_ptrs(s: CudaSampler, logits_ptr: int, dtype: int, B: int, 
     err = C.c_void_p()
     rc = s._lib.gorch_cuda_cross_entropy_bwd_dev(s._ctx, logits_ptr, dtype, B, V, row_stride, targets_ptr,
                                                  row_lse_ptr, float(scale), dx_ptr, dx_stride, C.byref(err))
+    _check(s._lib, rc, err)
+
+
+def distill_fwd_ptrs(s: CudaSampler, logits_ptr: int, dtype: int, B: int, V: int, row_stride: int, teacher_ids_ptr: int,
+                     teacher_logits_ptr: int, k: int, teacher_stride: int, temperature: float, row_loss_ptr: int, row_stats_ptr: int,
+                     mean_ptr: int | None = None) -> None:
+    """gorch_cuda_distill_fwd_dev: the loss of rows of logits against a teacher's k top logits (what topk leaves)."""
+    err = C.c_void_p()
+    rc = s._lib.gorch_cuda_distill_fwd_dev(s._ctx, logits_ptr, dtype, B, V, row_stride, teacher_ids_ptr, teacher_logits_ptr, k,
+                                           teacher_stride, float(temperature), row_loss_ptr, row_stats_ptr, mean_ptr, C.byref(err))
+    _check(s._lib, rc, err)
+
+
+def distill_bwd_ptrs(s: CudaSampler, logits_ptr: int, dtype: int, B: int, V: int, row_stride: int, teacher_ids_ptr: int,
+                     teacher_logits_ptr: int, k: int, teacher_stride: int, temperature: float, row_stats_ptr: int,
+                     row_grads_ptr: int | None, scale: float, accumulate: bool, dx_ptr: int, dx_stride: int) -> None:
+    """gorch_cuda_distill_bwd_dev: its gradient, written to dx or added to it."""
+    err = C.c_void_p()
+    rc = s._lib.gorch_cuda_distill_bwd_dev(s._ctx, logits_ptr, dtype, B, V, row_stride, teacher_ids_ptr, teacher_logits_ptr, k,
+                                           teacher_stride, float(temperature), row_stats_ptr, row_grads_ptr, float(scale),
+                                           1 if accumulate else 0, dx_ptr, dx_stride, C.byref(err))
     _check(s._lib, rc, err)
 
 
@@ -111,6 +133,61 @@ def cross_entropy_backward(s: CudaSampler, logits, targets, row_lse, scale: floa
     try:
         b_x, b_t, b_e, b_d = bufs.new(a), bufs.new(t), bufs.new(lse), bufs.new(dx.nbytes)
         cross_entropy_bwd_ptrs(s, bufs.ptr(b_x), dtype, B, V, V, bufs.ptr(b_t), bufs.ptr(b_e), scale, bufs.ptr(b_d), V)
+        s.sync()
+        if dx.nbytes:
+            s._download(b_d, dx)
+    finally:
+        bufs.free()
+    return dx
+
+
+def _teacher_arg(ids, values, B: int):
+    i = np.ascontiguousarray(ids, dtype=np.int32)
+    t = np.ascontiguousarray(values, dtype=np.float32)
+    if i.ndim != 2 or i.shape != t.shape or i.shape[0] != B:
+        raise ValueError("teacher ids and logits must be [B, k]")
+    return i, t
+
+
+def distill(s: CudaSampler, logits, teacher_ids, teacher_logits, temperature: float = 1.0):
+    """logits [B,V], the teacher's tokens and logits [B,k] (as `CudaSampler.topk` returns them; a token below 0 is no entry)
+    -> (mean loss, row_loss [B] f32, row_stats [B,4] f32)."""
+    a, dtype = _logits_arg(logits)
+    B, V = a.shape
+    i, t = _teacher_arg(teacher_ids, teacher_logits, B)
+    row_loss, stats, mean = np.empty(B, np.float32), np.empty((B, 4), np.float32), np.zeros(1, np.float32)
+    bufs = _Bufs(s)
+    try:
+        b_x, b_i, b_t = bufs.new(a), bufs.new(i), bufs.new(t)
+        b_l, b_s, b_m = bufs.new(4 * B), bufs.new(16 * B), bufs.new(mean)
+        distill_fwd_ptrs(s, bufs.ptr(b_x), dtype, B, V, V, bufs.ptr(b_i), bufs.ptr(b_t), i.shape[1], i.shape[1], temperature,
+                         bufs.ptr(b_l), bufs.ptr(b_s), bufs.ptr(b_m))
+        s.sync()
+        if B:
+            s._download(b_l, row_loss)
+            s._download(b_s, stats)
+            s._download(b_m, mean)
+    finally:
+        bufs.free()
+    return float(mean[0]), row_loss, stats
+
+
+def distill_backward(s: CudaSampler, logits, teacher_ids, teacher_logits, temperature: float, row_stats, row_grads=None,
+                     scale: float = 1.0, onto=None) -> np.ndarray:
+    """-> dx [B,V] float32: scale * row_grads times the gradient of each row's loss, added to `onto` where that is given."""
+    a, dtype = _logits_arg(logits)
+    B, V = a.shape
+    i, t = _teacher_arg(teacher_ids, teacher_logits, B)
+    stats = np.ascontiguousarray(row_stats, dtype=np.float32).reshape(B, 4)
+    grads = None if row_grads is None else np.ascontiguousarray(row_grads, dtype=np.float32).reshape(B)
+    dx = np.empty((B, V), dtype=np.float32) if onto is None else np.array(onto, dtype=np.float32).reshape(B, V)
+    bufs = _Bufs(s)
+    try:
+        b_x, b_i, b_t, b_s = bufs.new(a), bufs.new(i), bufs.new(t), bufs.new(stats)
+        b_g = None if grads is None else bufs.new(grads)
+        b_d = bufs.new(dx.nbytes if onto is None else dx)
+        distill_bwd_ptrs(s, bufs.ptr(b_x), dtype, B, V, V, bufs.ptr(b_i), bufs.ptr(b_t), i.shape[1], i.shape[1], temperature, bufs.ptr(b_s),
+                         None if b_g is None else bufs.ptr(b_g), scale, onto is not None, bufs.ptr(b_d), V)
         s.sync()
         if dx.nbytes:
             s._download(b_d, dx)

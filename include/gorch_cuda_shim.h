@@ -407,6 +407,31 @@ int gorch_cuda_cross_entropy_bwd_dev(GorchCudaCtxRef ctx, const void* logits, in
                                      const float* row_lse, float scale, float* dx,
                                      int64_t dx_stride, char** errOut);
 
+/* Distillation from a teacher's top logits, beside the cross-entropy (the reference trains on hard targets
+ * alone, loss.go:55-141); gorch_cuda_topk_dev makes the teacher's part. Row b's teacher is teacher_logits
+ * [B, teacher_stride] f32 and their tokens teacher_ids, k entries each, 1 <= k <= 16384; entries with
+ * a token outside [0, V) or a logit of -Inf are none. With p = softmax(teacher / T) over a row's entries and
+ * q = softmax(logits / T) over the vocabulary:
+ * gorch_cuda_distill_fwd_dev: row_loss[b] = T^2 sum_i p_i (log p_i - log q_i); mean_loss[0] = sum(row_loss) / B
+ * (may be NULL); row_stats [B][4] = (M, S, tM, tS), M = max x, S = sum exp((x - M) / T), tM and tS the same of
+ * the entries: what the backward pass needs. A row without entries (padding): loss 0, stats 0, and
+ * its logits are not read. A token listed twice counts as two entries.
+ * gorch_cuda_distill_bwd_dev: dx[b,j] = scale * row_grads[b] * T * (q_j - p of token j), f32 [B,dx_stride];
+ * row_grads may be NULL (1); accumulate != 0: added to what dx holds (rows without entries stay as
+ * they are; otherwise they become 0), which puts this gradient on top of gorch_cuda_cross_entropy_bwd_dev's. dx may be
+ * the logits themselves if those are f32 with the same stride (accumulate 0), and must not overlap them otherwise.
+ * The temperature lies in 1e-6 .. 1e6. NaN, +Inf or nothing but -Inf in a taught row makes its loss and gradient
+ * NaN; an entry whose logit in x is -Inf makes the loss +Inf, and the gradient stays finite. */
+int gorch_cuda_distill_fwd_dev(GorchCudaCtxRef ctx, const void* logits, int dtype, int64_t B, int64_t V,
+                               int64_t row_stride, const int32_t* teacher_ids, const float* teacher_logits,
+                               int64_t k, int64_t teacher_stride, float temperature, float* row_loss,
+                               float* row_stats, float* mean_loss, char** errOut);
+int gorch_cuda_distill_bwd_dev(GorchCudaCtxRef ctx, const void* logits, int dtype, int64_t B, int64_t V,
+                               int64_t row_stride, const int32_t* teacher_ids, const float* teacher_logits,
+                               int64_t k, int64_t teacher_stride, float temperature,
+                               const float* row_stats, const float* row_grads, float scale,
+                               int accumulate, float* dx, int64_t dx_stride, char** errOut);
+
 /* The LM-head projection that produces the logits: logits[b, v] = sum_k x[b, k] * w[v, k], i.e.
  * MatMulTransB(last, m.Embed.Weight) of model/qwen/qwen.go:80-85 (GPT-2: nn/gpt.go:119-120; the CPU
  * loop is nn/extembed.go:152-195), for x [B, K] and w [V, K] in bf16 (bit patterns, row pitches ldx /
