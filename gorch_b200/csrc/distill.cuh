@@ -9,7 +9,8 @@
 // The forward pass leaves (M, S, tM, tS) for the backward pass, and not log S: exp((x - M) / T) / S is as exact as its f32 parts,
 // where a rounded M / T + log S would put 1e-6 of relative error on every q.
 //
-// Bound: memory. Forward reads x once, backward reads x and writes the f32 gradient once.
+// Bound: memory. Forward reads x once (1,500 x 168,320 f32, a twentieth of the rows without entries: 192 us, 5.0 TB/s), backward reads x
+// and writes the f32 gradient once (329 us, 6.0 TB/s).
 #pragma once
 
 #include <cooperative_groups.h>
@@ -20,12 +21,14 @@
 
 namespace gs {
 
-constexpr int DF_NT = 512;
-constexpr int DF_U = 8;                       // 16-byte loads of a thread that are on their way together
+constexpr int DF_NT = 256;
+constexpr int DF_PER_SM = 4;                  // CTAs of 64 registers a thread
+constexpr int DF_U = 8;                       // 16-byte loads of a thread that are on their way together (us, loads x CTAs per SM: 4 x 6: 220, 6 x 5: 193,
+                                              // 8 x 4: 192, 8 x 3: 245)
 constexpr int DF_MAX_C = 8;                   // CTAs per row
 constexpr int DB_NT = 256;
-constexpr int DB_U = 4;                       // vectors of a thread, all of them on their way at once
-constexpr int DB_LIST = 256;                  // a CTA's entries that are kept in shared memory
+constexpr int DB_U = 4;                       // 16-byte vectors of a thread that are on their way together
+constexpr int DB_MAX_P = 8;                   // batches of them that a CTA takes at most
 constexpr float DS_MIN_T = 1e-6f, DS_MAX_T = 1e6f;
 
 // exp(x / T) = 2^(x log2(e) / T): log2(e) / T to f32 and what that leaves out, and where exp(x / T) is 0 in f32.
@@ -56,7 +59,7 @@ struct DistillArgs {
   int32_t accumulate;
   float* dx;                  // [B, dx_stride]
   int64_t dx_stride;
-  int32_t nchunk;             // backward: CTAs per row
+  int32_t nchunk, batches;    // backward: CTAs per row, batches of vectors each
 };
 
 // exp(d / T) of two d <= 0: as rs_exp2, with the temperature in the constants. (Below the floor the result is 0 all the same, and an
@@ -76,15 +79,17 @@ __device__ __forceinline__ rs_f2 ds_exp2(float d0, float d1, const DsScale& s) {
 __device__ __forceinline__ bool ds_entry(int id, float t, int V) { return id >= 0 && id < V && !(t == -INFINITY); }
 
 // A cluster of C CTAs takes a row, each a slice of it. Every thread keeps a running maximum m and the sum of exp((x - m) / T) over its
-// own elements, rescaled when m grows; the terms' precision is that of rs_max_sum (row_softmax.cuh). The first CTA adds up
-// the teacher's side while its first logits are on their way.
+// own elements, rescaled when m grows (the terms' precision is that of rs_max_sum, row_softmax.cuh). In the first CTA the
+// threads do the same with the teacher's entries, and for the sums of p times t and x. So a row costs one reduction at its end,
+// and its first logits are asked for before anything is known of it but that its first entry is one.
 template <typename T>
-__global__ void __launch_bounds__(DF_NT, 2) distill_fwd_kernel(const __grid_constant__ DistillArgs A) {
+__global__ void __launch_bounds__(DF_NT, DF_PER_SM) distill_fwd_kernel(const __grid_constant__ DistillArgs A) {
   namespace cg = cooperative_groups;
   constexpr int VEC = Elem<T>::VEC, NW = DF_NT / 32, U = DF_U;
   __shared__ bu::Scratch sc;
+  __shared__ double s_sum[4][NW];
   __shared__ RsHalf xch[DF_MAX_C];
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   cg::cluster_group cluster = cg::this_cluster();
   const int C = static_cast<int>(cluster.num_blocks());
   const int rank = static_cast<int>(cluster.block_rank());
@@ -98,21 +103,16 @@ __global__ void __launch_bounds__(DF_NT, 2) distill_fwd_kernel(const __grid_cons
   const int v0 = min(rank * per, rv.nvec), v1 = min(v0 + per, rv.nvec);
   const int32_t* ids = A.ids + row * A.t_stride;
   const float* tea = A.teacher + row * A.t_stride;
-  float tm = -INFINITY;
-  bool tnan = false, some = false;
-  for (int i = tid; i < A.k; i += DF_NT) {
-    const float t = __ldg(tea + i);
-    if (!ds_entry(__ldg(ids + i), t, A.V)) continue;
-    some = true;
-    tnan |= t != t;
-    tm = fmaxf(tm, t);
-  }
-  if (!__syncthreads_or(some)) {                               // (every CTA of the cluster comes to the same)
-    if (rank == 0 && tid == 0) {
-      A.row_loss[row] = 0.0f;
-      for (int i = 0; i < 4; i++) A.stats[4 * row + i] = 0.0f;
+  if (!ds_entry(__ldg(ids), __ldg(tea), A.V)) {                // perhaps a row without entries
+    bool some = false;
+    for (int i = tid; i < A.k; i += DF_NT) some |= ds_entry(__ldg(ids + i), __ldg(tea + i), A.V);
+    if (!__syncthreads_or(some)) {                             // (every CTA of the cluster comes to the same)
+      if (rank == 0 && tid == 0) {
+        A.row_loss[row] = 0.0f;
+        for (int i = 0; i < 4; i++) A.stats[4 * row + i] = 0.0f;
+      }
+      return;
     }
-    return;
   }
   uint4 raw[U];
   auto load = [&](int v) {
@@ -121,21 +121,6 @@ __global__ void __launch_bounds__(DF_NT, 2) distill_fwd_kernel(const __grid_cons
   };
   load(v0 + tid);
   if (C > 1) cluster.barrier_arrive();
-  double ts = 0.0, at = 0.0, ax = 0.0;                         // sums of exp((t - tM) / T), and of it times t - tM and x
-  if (rank == 0) {
-    tm = okey_to_float(static_cast<uint32_t>(bu::max_u64<NW>(static_cast<unsigned long long>(okey(tm)), sc, tid)));
-    if (tnan) ts = __longlong_as_double(0x7ff8000000000000ll);
-    for (int i = tid; i < A.k; i += DF_NT) {
-      const float t = __ldg(tea + i);
-      const int id = __ldg(ids + i);
-      if (!ds_entry(id, t, A.V)) continue;
-      const float d = t - tm;                                  // (t = tM = Inf: NaN, and so is the row)
-      const double e = static_cast<double>(expf(__fdiv_rn(d, A.T)));
-      ts += e;
-      if (e != 0.0) { at += e * static_cast<double>(d); ax += e * static_cast<double>(Elem<T>::to_float(xrow[id])); }
-    }
-    bu::sum_d3<NW>(ts, at, ax, sc, tid);
-  }
   float m = -INFINITY;
   rs_f2 s2 = rs_pk(0.0f, 0.0f);
   const float c = A.sc.hi;
@@ -169,11 +154,50 @@ __global__ void __launch_bounds__(DF_NT, 2) distill_fwd_kernel(const __grid_cons
     }
     load(va + U * DF_NT);
   }
-  float M = okey_to_float(static_cast<uint32_t>(bu::max_u64<NW>(static_cast<unsigned long long>(okey(m)), sc, tid)));
+  // the teacher's side: sums of e = exp((t - own maximum) / T), of e (t - own maximum) and of e x
+  float tm = -INFINITY;
+  double ts = 0.0, at = 0.0, ax = 0.0;
+  if (rank == 0) {
+    for (int i = tid; i < A.k; i += DF_NT) {
+      const float t = __ldg(tea + i);
+      const int id = __ldg(ids + i);
+      if (!ds_entry(id, t, A.V)) continue;
+      const double x = static_cast<double>(Elem<T>::to_float(__ldg(xrow + id)));
+      if (t > tm) {
+        const double d = static_cast<double>(tm) - static_cast<double>(t), f = static_cast<double>(expf(static_cast<float>(d / static_cast<double>(A.T))));
+        if (f > 0.0) { at = f * (at + ts * d); ax *= f; } else { at = 0.0; ax = 0.0; }   // (what is 0 in f32 is no term: not 0 times Inf)
+        ts = ts * f + 1.0;
+        ax += x;
+        tm = t;
+      } else {
+        const float d = t - tm;                                // (NaN or Inf: the row becomes NaN)
+        const double e = static_cast<double>(expf(__fdiv_rn(d, A.T)));
+        ts += e;
+        if (e != 0.0) { at += e * static_cast<double>(d); ax += e * x; }
+      }
+    }
+  }
+  // the row's maxima, then its sums
+  uint32_t km = okey(m), kt = okey(tm), unused = 0u;
+  bu::max_u3<NW>(km, kt, unused, sc, tid);
+  float M = okey_to_float(km);
+  const float tM = okey_to_float(kt);
   float sa, sb;
   rs_upk(s2, sa, sb);
   const float s = sa + sb;
-  double S = bu::sum_d<NW>((m > -INFINITY || s != s) ? static_cast<double>(s) * static_cast<double>(expf(__fdiv_rn((m > -INFINITY ? m : M) - M, A.T))) : 0.0, sc, tid);
+  double sum = (m > -INFINITY || s != s) ? static_cast<double>(s) * static_cast<double>(expf(__fdiv_rn((m > -INFINITY ? m : M) - M, A.T))) : 0.0;
+  sum = warp_sum_d(sum);
+  const bool warp_teaches = rank == 0 && warp * 32 < A.k;
+  if (warp_teaches) {
+    const double d = static_cast<double>(tm) - static_cast<double>(tM);
+    const double f = ts == 0.0 ? 0.0 : static_cast<double>(expf(static_cast<float>(d / static_cast<double>(A.T))));
+    if (f == 0.0) { ts = 0.0; at = 0.0; ax = 0.0; } else { at = f * (at + ts * d); ax *= f; ts *= f; }
+    ts = warp_sum_d(ts); at = warp_sum_d(at); ax = warp_sum_d(ax);
+  }
+  if (lane == 0) { s_sum[0][warp] = sum; s_sum[1][warp] = warp_teaches ? ts : 0.0; s_sum[2][warp] = warp_teaches ? at : 0.0; s_sum[3][warp] = warp_teaches ? ax : 0.0; }
+  __syncthreads();
+  double S = 0.0;
+  for (int w = 0; w < NW; w++) S += s_sum[0][w];
   if (C > 1) {
     cluster.barrier_wait();
     if (tid == 0) { RsHalf* p = cluster.map_shared_rank(&xch[rank], 0); p->m = M; p->s = S; }
@@ -189,50 +213,53 @@ __global__ void __launch_bounds__(DF_NT, 2) distill_fwd_kernel(const __grid_cons
     M = Mt;
     S = St;
   }
-  if (rank == 0 && tid == 0) {
+  if (tid == 0) {
     if (!(M > -INFINITY)) S = __longlong_as_double(0x7ff8000000000000ll);   // a row of -Inf only
+    ts = at = ax = 0.0;
+    for (int w = 0; w < NW; w++) { ts += s_sum[1][w]; at += s_sum[2][w]; ax += s_sum[3][w]; }
     const double Td = static_cast<double>(A.T);
     A.row_loss[row] = static_cast<float>(Td * (at / ts - (ax / ts - static_cast<double>(M))) + Td * Td * (log(S) - log(ts)));
     A.stats[4 * row] = M;
     A.stats[4 * row + 1] = static_cast<float>(S);
-    A.stats[4 * row + 2] = tm;
+    A.stats[4 * row + 2] = tM;
     A.stats[4 * row + 3] = static_cast<float>(ts);
   }
 }
 
-// A CTA takes DB_NT x DB_U vectors of a row. The teacher's entries that fall among them are few: a bit per column says
-// whether a column has one, and such a column looks through the list of the CTA's entries.
+// A CTA takes A.batches x DB_NT x DB_U vectors of a row. The teacher's entries that fall among them are few: a bit per column says
+// whether a column has one; such columns are left out of the stream and finished behind it, an entry per thread. A column
+// whose token is listed more than once (which a bit that is already there shows) is finished by its first entry, with the
+// others' probabilities added in the list's order. (With the lookup inside the stream, a call there: 401 us for 1,500 x 168,320 f32.)
 template <typename T>
-__global__ void __launch_bounds__(DB_NT) distill_bwd_kernel(const __grid_constant__ DistillArgs A) {
+__global__ void __launch_bounds__(DB_NT, 4) distill_bwd_kernel(const __grid_constant__ DistillArgs A) {
   constexpr int VEC = Elem<T>::VEC, U = DB_U, COLS = DB_NT * U * VEC;
-  __shared__ uint32_t s_bits[COLS / 32];
-  __shared__ int s_at[DB_LIST], s_id[DB_LIST];                 // number of the entry, its token
-  __shared__ int s_n;
+  __shared__ uint32_t s_bits[DB_MAX_P * COLS / 32];
+  __shared__ int s_any, s_twice;
   const int tid = threadIdx.x;
   const int64_t row = blockIdx.x / static_cast<unsigned>(A.nchunk);
   const int part = static_cast<int>(blockIdx.x - static_cast<unsigned>(row) * static_cast<unsigned>(A.nchunk));
-  for (int i = tid; i < COLS / 32; i += DB_NT) s_bits[i] = 0u;
-  if (tid == 0) s_n = 0;
+  for (int i = tid; i < A.batches * (COLS / 32); i += DB_NT) s_bits[i] = 0u;
+  if (tid == 0) { s_any = 0; s_twice = 0; }
   pdl_launch();
   pdl_wait();                                                  // the forward pass
   const T* xrow = static_cast<const T*>(A.x) + row * A.row_stride;
   float* drow = A.dx + row * A.dx_stride;
   RowView<T> rv;
   rv.init(xrow, A.V);
-  const int v0 = part * (DB_NT * U);
-  if (v0 >= rv.nvec) return;
+  const int v0 = part * A.batches * (DB_NT * U), v1 = min(v0 + A.batches * (DB_NT * U), rv.nvec);
+  if (v0 >= v1) return;
   const float M = A.stats[4 * row], S = A.stats[4 * row + 1], tM = A.stats[4 * row + 2], tS = A.stats[4 * row + 3];
   const float g = A.row_grads ? A.row_grads[row] : 1.0f;
   const bool none = tS == 0.0f;
   if (none && A.accumulate) return;
   uint4 raw[U];
+  auto load = [&](int v) {
 #pragma unroll
-  for (int u = 0; u < U; u++) {
-    const int v = v0 + u * DB_NT + tid;
-    raw[u] = (!none && v < rv.nvec) ? *(rv.vbase + v) : make_uint4(0u, 0u, 0u, 0u);   // (dx may lie where x lies)
-  }
+    for (int u = 0; u < U; u++) raw[u] = (!none && v + u * DB_NT < v1) ? *(rv.vbase + v + u * DB_NT) : make_uint4(0u, 0u, 0u, 0u);   // (dx may lie where x lies)
+  };
+  load(v0 + tid);
   const int c0 = v0 * VEC - rv.shift;                          // column of the first element: below 0 in a row's first vector
-  const int lo = max(c0, 0), hi = min(c0 + COLS, A.V);
+  const int lo = max(c0, 0), hi = min(v1 * VEC - rv.shift, A.V);
   const int32_t* ids = A.ids + row * A.t_stride;
   const float* tea = A.teacher + row * A.t_stride;
   __syncthreads();
@@ -240,54 +267,67 @@ __global__ void __launch_bounds__(DB_NT) distill_bwd_kernel(const __grid_constan
     for (int i = tid; i < A.k; i += DB_NT) {
       const int id = __ldg(ids + i);
       if (id < lo || id >= hi || __ldg(tea + i) == -INFINITY) continue;
-      atomicOr(&s_bits[(id - c0) >> 5], 1u << ((id - c0) & 31));
-      const int at = atomicAdd(&s_n, 1);
-      if (at < DB_LIST) { s_at[at] = i; s_id[at] = id; }
+      const uint32_t bit = 1u << ((id - c0) & 31);
+      if (atomicOr(&s_bits[(id - c0) >> 5], bit) & bit) s_twice = 1;
+      s_any = 1;
     }
   }
   __syncthreads();
-  const int n = s_n;
+  const bool any = s_any != 0, twice = s_twice != 0;
   const float coef = none ? 0.0f : static_cast<float>(static_cast<double>(A.scale) * static_cast<double>(g) * static_cast<double>(A.T));
   const float inv = none ? 0.0f : 1.0f / S;
-  // the teacher's probability of a column: its entries' in the order of the list they came in
-  auto teacher = [&](int col) -> float {
-    float p = 0.0f;
-    if (n <= DB_LIST) {
-      for (int after = -1;;) {
-        int next = A.k;
-        for (int j = 0; j < n; j++) if (s_id[j] == col && s_at[j] > after) next = min(next, s_at[j]);
-        if (next == A.k) return p;
-        p += expf(__fdiv_rn(__ldg(tea + next) - tM, A.T)) / tS;
-        after = next;
+  const bool vec_ok = ((reinterpret_cast<uintptr_t>(drow) - static_cast<uintptr_t>(rv.shift) * 4u) & 15u) == 0;
+  for (int va = v0 + tid; va < v1; va += U * DB_NT) {
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const int v = va + u * DB_NT, i0 = v * VEC - rv.shift, e0 = (v - v0) * VEC;
+      if (v >= v1) break;
+      float x[VEC], y[VEC];
+      Elem<T>::unpack(raw[u], x);
+#pragma unroll
+      for (int c = 0; c < VEC; c += 2) {
+        const rs_f2 q = rs_mul2(ds_exp2(x[c] - M, x[c + 1] - M, A.sc), rs_pk(inv, inv));
+        rs_upk(rs_mul2(q, rs_pk(coef, coef)), y[c], y[c + 1]);
+      }
+      if (none) {
+#pragma unroll
+        for (int c = 0; c < VEC; c++) y[c] = 0.0f;
+      }
+      if (A.accumulate) {
+#pragma unroll
+        for (int c = 0; c < VEC; c++) if (i0 + c >= 0 && i0 + c < A.V) y[c] += drow[i0 + c];
+      }
+      const uint32_t bits = any ? (s_bits[e0 >> 5] >> (e0 & 31)) & ((1u << VEC) - 1u) : 0u;
+      if (bits == 0u) {
+        rs_store<float, VEC>(drow, vec_ok, A.V, i0, y);
+      } else {
+#pragma unroll
+        for (int c = 0; c < VEC; c++) if (!((bits >> c) & 1u) && i0 + c >= 0 && i0 + c < A.V) drow[i0 + c] = y[c];
       }
     }
-    for (int i = 0; i < A.k; i++) if (__ldg(ids + i) == col && !(__ldg(tea + i) == -INFINITY)) p += expf(__fdiv_rn(__ldg(tea + i) - tM, A.T)) / tS;
-    return p;
-  };
-  const bool vec_ok = ((reinterpret_cast<uintptr_t>(drow) - static_cast<uintptr_t>(rv.shift) * 4u) & 15u) == 0;
-#pragma unroll
-  for (int u = 0; u < U; u++) {
-    const int v = v0 + u * DB_NT + tid, i0 = v * VEC - rv.shift, e0 = (u * DB_NT + tid) * VEC;
-    if (v >= rv.nvec) break;
-    float x[VEC], y[VEC];
-    Elem<T>::unpack(raw[u], x);
-#pragma unroll
-    for (int c = 0; c < VEC; c += 2) rs_upk(rs_mul2(ds_exp2(x[c] - M, x[c + 1] - M, A.sc), rs_pk(inv, inv)), y[c], y[c + 1]);
-    uint32_t bits = (n > 0) ? (s_bits[e0 >> 5] >> (e0 & 31)) & ((1u << VEC) - 1u) : 0u;
-    while (bits) {
-      const int c = __ffs(bits) - 1;
-      bits &= bits - 1u;
-      const float p = teacher(i0 + c);
-#pragma unroll
-      for (int j = 0; j < VEC; j++) if (j == c) y[j] -= p;
+    load(va + U * DB_NT);
+  }
+  if (!any) return;
+  for (int i = tid; i < A.k; i += DB_NT) {
+    const int id = __ldg(ids + i);
+    if (id < lo || id >= hi) continue;
+    const float t = __ldg(tea + i);
+    if (t == -INFINITY) continue;
+    float p = expf(__fdiv_rn(t - tM, A.T)) / tS;
+    if (twice) {
+      bool first = true;
+      for (int j = 0; j < A.k && first; j++) {
+        if (j == i || __ldg(ids + j) != id || __ldg(tea + j) == -INFINITY) continue;
+        if (j < i) first = false;
+        else p += expf(__fdiv_rn(__ldg(tea + j) - tM, A.T)) / tS;
+      }
+      if (!first) continue;
     }
-#pragma unroll
-    for (int c = 0; c < VEC; c++) y[c] = none ? 0.0f : y[c] * coef;
-    if (A.accumulate) {
-#pragma unroll
-      for (int c = 0; c < VEC; c++) if (i0 + c >= 0 && i0 + c < A.V) y[c] += drow[i0 + c];
-    }
-    rs_store<float, VEC>(drow, vec_ok, A.V, i0, y);
+    float q, unused;
+    const float d = Elem<T>::to_float(xrow[id]) - M;           // (left alone by the stream, where dx lies over x)
+    rs_upk(rs_mul2(ds_exp2(d, d, A.sc), rs_pk(inv, inv)), q, unused);
+    const float y = (q - p) * coef;
+    drow[id] = A.accumulate ? y + drow[id] : y;
   }
 }
 
