@@ -28,6 +28,7 @@ EXPORTS = [
     "gorch_cuda_adjust_logits_dev", "gorch_cuda_generate_step_adjusted_dev",
     "gorch_cuda_softmax_dev", "gorch_cuda_cross_entropy_fwd_dev", "gorch_cuda_cross_entropy_bwd_dev",
     "gorch_cuda_distill_fwd_dev", "gorch_cuda_distill_bwd_dev",
+    "gorch_cuda_lm_head_adapters_workspace", "gorch_cuda_lm_head_adapters_dev",
 ]
 
 
@@ -50,6 +51,14 @@ class LogitAdjust(C.Structure):
         ("penalties", C.c_void_p), ("history", C.c_void_p), ("history_stride", C.c_int64), ("history_lengths", C.c_void_p),
         ("prompt_lengths", C.c_void_p), ("bias_offsets", C.c_void_p), ("bias_ids", C.c_void_p), ("bias_values", C.c_void_p),
         ("n_bias", C.c_int64), ("mask", C.c_void_p), ("mask_stride", C.c_int64), ("n_masks", C.c_int64), ("mask_rows", C.c_void_p),
+    ]
+
+
+class Adapters(C.Structure):
+    """GorchAdapters of include/gorch_cuda_shim.h (device pointers; pitches and strides in elements)."""
+    _fields_ = [
+        ("a", C.c_void_p), ("a_pitch", C.c_int64), ("a_stride", C.c_int64), ("b", C.c_void_p), ("b_pitch", C.c_int64),
+        ("b_stride", C.c_int64), ("scales", C.c_void_p), ("n", C.c_int64), ("rank", C.c_int64),
     ]
 
 
@@ -111,6 +120,8 @@ def load() -> C.CDLL:
         "gorch_cuda_lm_head_logits_dev": (i32, [p, p, i64, p, i64, i64, i64, i64, p, i64, err]),
         "gorch_cuda_lm_head_status": (i32, [p, C.POINTER(C.c_uint32), err]),
         "gorch_cuda_lm_head_sample_dev": (i32, [p, p, i64, p, i64, i64, i64, i64, i32, p, p, p, p, err]),
+        "gorch_cuda_lm_head_adapters_workspace": (i32, [i64, C.POINTER(Adapters), C.POINTER(C.c_uint64), err]),
+        "gorch_cuda_lm_head_adapters_dev": (i32, [p, p, i64, p, i64, i64, i64, i64, C.POINTER(Adapters), p, p, C.c_uint64, p, i64, err]),
         "gorch_cuda_topk_dev": (i32, [p, p, i32, i64, i64, i64, i64, p, p, p, err]),
         "gorch_cuda_multinomial_dev": (i32, [p, p, i64, i64, i64, p, p, p, err]),
         "gorch_cuda_softmax_dev": (i32, [p, p, i32, i64, i64, i64, p, i64, i32, err]),

@@ -37,6 +37,7 @@
 
 #include <cuda.h>
 
+#include "row_softmax.cuh"     // bf16_bits_rne
 #include "sample_batch.cuh"
 
 namespace gs {
@@ -89,6 +90,158 @@ struct LmHeadArgs {
   int32_t clear_status;    // 1: this launch clears it first
   int32_t chained;         // 1: launched as a dependent of the kernel that fills thr, with x and w there before; 0: of any kernel
 };
+
+// ---- low-rank adapters beside the projection -----------------------------------------------------------
+// logits[b, v] += h[b] . b[a][v], h[b] = scale[a] * (a[a] x[b]), for the adapter a that row b has (none: no term). For the tensor pipe
+// these are further columns of K: for every adapter that a group of item_n batch rows uses, its b [V, rank] on the w side, and
+// on the x side h in the rows that use it and 0 in the others. So the products of an item go on, after K, over the group's
+// adapters in units of LMA_UNIT columns of the rank, LMA_STAGE of them in a stage of the ring (32-byte rows, 32-byte swizzle; what a
+// rank leaves of a unit is filled with zeros by the copy). The rows need no order, every adapter's b passes once per
+// batch group, and the epilogue's results are complete. h goes in as two bf16, the rounded value and what the rounding left (2^-16 of
+// it is lost at most, about what the f32 sums over K lose), each multiplied with the same tile of b: one bf16 would put 2^-9 of
+// the adapter's term on logits that are f32.
+// 0 times an Inf or NaN in an adapter's b is NaN, in rows that do not use that adapter too (and the two parts of h may disagree about an
+// Inf in the row's own): where a group has adapters, the epilogue works a NaN out again from the row's own operands, unless x holds one.
+constexpr int LMA_UNIT = 16;             // columns of the rank in a unit: K of one MMA, 32 bytes
+constexpr int LMA_STAGE = 4;             // units in a stage
+constexpr int LMA_MAX_RANK = 256;
+constexpr int LMA_NT = 256;              // of the kernel that makes h
+constexpr int LMA_HDR = 4;               // words of a group's record ahead of its adapters: the first one says how many
+static_assert(LMA_STAGE * 2 * 32 <= LMH_SUB * LMH_BK * 2 && LMA_STAGE * LMH_CTA_V * 32 <= LMH_SUB * LMH_W_BYTES, "a stage holds its units");
+
+struct LmAdaptArgs {
+  CUtensorMap map_b;       // b [n, V, rank] bf16, box 16 x cta_v, 32-byte swizzle
+  CUtensorMap map_h;       // h [group][unit][2][item_n] rows of 16 bf16, box 16 x box_n, 32-byte swizzle
+  const uint16_t *x, *w, *a, *b;
+  int64_t ldx, ldw, a_pitch, a_stride, b_pitch, b_stride;   // in elements
+  const float* scales;     // [n] or null: 1
+  const int32_t* row_adapter;   // [B]; outside [0, n): none
+  int32_t n, rank, units;  // adapters, their rank, units of one
+  int32_t max_units;       // of a group
+  int32_t* groups;         // [group][LMA_HDR + item_n]
+  int32_t* row_nan;        // [B]
+  uint16_t* h;
+};
+__host__ __device__ inline int64_t lma_h_row(const LmAdaptArgs& D, int item_n, int group, int unit, int piece, int row) {
+  return ((static_cast<int64_t>(group) * D.max_units + unit) * 2 + piece) * item_n + row;
+}
+
+__device__ __forceinline__ float bf16_lo(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float bf16_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+
+// A CTA per batch row: which adapters its group uses (in the order of their first rows), and its h for all of them.
+__global__ void __launch_bounds__(LMA_NT) lm_adapters_kernel(const __grid_constant__ LmAdaptArgs D, const int32_t B, const int32_t K, const int32_t item_n) {
+  __shared__ __align__(16) int s_ad[LMA_NT];
+  __shared__ int s_first[LMA_NT / 32], s_mine;
+  __shared__ float s_h[LMA_MAX_RANK];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int b = blockIdx.x, g = b / item_n, g0 = g * item_n, rows = min(item_n, B - g0);
+  pdl_launch();
+  int a = (tid < rows) ? D.row_adapter[g0 + tid] : -1;
+  if (a < 0 || a >= D.n) a = -1;
+  s_ad[tid] = a;
+  if (tid == 0) s_mine = -1;
+  __syncthreads();
+  bool first = a >= 0;
+#pragma unroll 4
+  for (int j = 0; j < tid; j += 4) {
+    const int4 o = *reinterpret_cast<const int4*>(&s_ad[j]);
+    if (o.x == a || (o.y == a && j + 1 < tid) || (o.z == a && j + 2 < tid) || (o.w == a && j + 3 < tid)) first = false;
+  }
+  const uint32_t votes = __ballot_sync(FULL, first);
+  if (lane == 0) s_first[warp] = __popc(votes);
+  __syncthreads();
+  const int mine = s_ad[b - g0];
+  int slot = __popc(votes & ((1u << lane) - 1u)), nslots = 0;
+  for (int w = 0; w < LMA_NT / 32; w++) { slot += w < warp ? s_first[w] : 0; nslots += s_first[w]; }
+  if (first && a == mine) s_mine = slot;
+  int32_t* rec = D.groups + static_cast<int64_t>(g) * (LMA_HDR + item_n);
+  __syncthreads();                                                   // s_mine
+  if (b == g0) {
+    if (first) rec[LMA_HDR + slot] = a;
+    if (tid == 0) rec[0] = nslots;
+  }
+  // h = scale * a x, a rank's row per warp
+  const uint4* x4 = reinterpret_cast<const uint4*>(D.x + b * D.ldx);
+  const int nk = K / 8;
+  bool nan = false;
+  if (mine >= 0) {
+    const float scale = D.scales ? D.scales[mine] : 1.0f;
+    for (int r = warp; r < D.rank; r += LMA_NT / 32) {
+      const uint4* a4 = reinterpret_cast<const uint4*>(D.a + mine * D.a_stride + r * D.a_pitch);
+      float acc = 0.0f;
+#pragma unroll 4
+      for (int k = lane; k < nk; k += 32) {
+        const uint4 p = __ldg(x4 + k), q = __ldg(a4 + k);
+        acc = fmaf(bf16_lo(p.x), bf16_lo(q.x), acc); acc = fmaf(bf16_hi(p.x), bf16_hi(q.x), acc);
+        acc = fmaf(bf16_lo(p.y), bf16_lo(q.y), acc); acc = fmaf(bf16_hi(p.y), bf16_hi(q.y), acc);
+        acc = fmaf(bf16_lo(p.z), bf16_lo(q.z), acc); acc = fmaf(bf16_hi(p.z), bf16_hi(q.z), acc);
+        acc = fmaf(bf16_lo(p.w), bf16_lo(q.w), acc); acc = fmaf(bf16_hi(p.w), bf16_hi(q.w), acc);
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(FULL, acc, o);
+      if (lane == 0) s_h[r] = acc * scale;
+    }
+  }
+  for (int k = tid; k < nk; k += LMA_NT) {
+    const uint4 p = __ldg(x4 + k);
+    const float t = (bf16_lo(p.x) * 0.0f + bf16_hi(p.x) * 0.0f) + (bf16_lo(p.y) * 0.0f + bf16_hi(p.y) * 0.0f) + (bf16_lo(p.z) * 0.0f + bf16_hi(p.z) * 0.0f) +
+                    (bf16_lo(p.w) * 0.0f + bf16_hi(p.w) * 0.0f);
+    if (t != t) {                                                    // a NaN or an infinity
+      const uint32_t ws[4] = {p.x, p.y, p.z, p.w};
+      for (int c = 0; c < 4; c++) nan |= bf16_lo(ws[c]) != bf16_lo(ws[c]) || bf16_hi(ws[c]) != bf16_hi(ws[c]);
+    }
+  }
+  const int any = __syncthreads_or(nan);                             // (and s_h is there)
+  if (tid == 0) D.row_nan[b] = any;
+  // 16 bytes at a time: of every unit's row of this batch row, half of either piece
+  for (int i = tid; i < nslots * D.units * 4; i += LMA_NT) {
+    const int unit = i >> 2, piece = (i >> 1) & 1, half = i & 1;
+    uint32_t o[4] = {0u, 0u, 0u, 0u};
+    if (unit / D.units == s_mine) {
+      const int r0 = (unit % D.units) * LMA_UNIT + half * 8;
+#pragma unroll
+      for (int c = 0; c < 8; c++) {
+        const float v = (r0 + c < D.rank) ? s_h[r0 + c] : 0.0f;
+        const uint32_t top = bf16_bits_rne(v);
+        const float left = v - __uint_as_float(top << 16);
+        // (an infinity's, and a NaN's, are in the rounded value)
+        const uint32_t bits = piece == 0 ? top : (fabsf(__uint_as_float(top << 16)) < INFINITY ? bf16_bits_rne(left) : 0u);
+        o[c >> 1] |= bits << (16 * (c & 1));
+      }
+    }
+    uint4* dst = reinterpret_cast<uint4*>(D.h + lma_h_row(D, item_n, g, unit, piece, b - g0) * LMA_UNIT) + half;
+    *dst = make_uint4(o[0], o[1], o[2], o[3]);
+  }
+}
+
+// One logit from its row's own operands, in f32.
+__device__ __noinline__ float lma_logit(const LmAdaptArgs& D, int K, int item_n, int b, int v) {
+  const uint4 *x4 = reinterpret_cast<const uint4*>(D.x + b * D.ldx), *w4 = reinterpret_cast<const uint4*>(D.w + v * D.ldw);
+  float acc = 0.0f;
+  for (int k = 0; k < K / 8; k++) {
+    const uint4 p = __ldg(x4 + k), q = __ldg(w4 + k);
+    const uint32_t ps[4] = {p.x, p.y, p.z, p.w}, qs[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int c = 0; c < 4; c++) { acc = fmaf(bf16_lo(ps[c]), bf16_lo(qs[c]), acc); acc = fmaf(bf16_hi(ps[c]), bf16_hi(qs[c]), acc); }
+  }
+  const int a = D.row_adapter[b];
+  if (a < 0 || a >= D.n) return acc;
+  const int g = b / item_n;
+  const int32_t* rec = D.groups + static_cast<int64_t>(g) * (LMA_HDR + item_n);
+  int slot = 0;
+  while (slot < rec[0] - 1 && rec[LMA_HDR + slot] != a) slot++;
+  const uint16_t* brow = D.b + a * D.b_stride + v * D.b_pitch;
+  for (int r = 0; r < D.rank; r++) {
+    const int unit = slot * D.units + r / LMA_UNIT;
+    float h = 0.0f;                                                    // (the two parts' sum is exact)
+#pragma unroll
+    for (int piece = 0; piece < 2; piece++)
+      h += __uint_as_float(static_cast<uint32_t>(D.h[lma_h_row(D, item_n, g, unit, piece, b - g * item_n) * LMA_UNIT + r % LMA_UNIT]) << 16);
+    acc = fmaf(h, __uint_as_float(static_cast<uint32_t>(__ldg(brow + r)) << 16), acc);
+  }
+  return acc;
+}
 
 // Work items in the order in which pair p takes them: p, p + npairs, ...: first the whole rounds of full
 // items (all batch rows of `full` vocabulary tiles, item_n at a time), then the remaining tiles in items
@@ -160,6 +313,14 @@ __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap
 __device__ __forceinline__ uint64_t umma_desc(uint32_t smem_addr_bytes) {
   return static_cast<uint64_t>((smem_addr_bytes & 0x3ffffu) >> 4) | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
 }
+// The same for 32-byte rows with the 32-byte swizzle: eight rows are 256 bytes, layout type 6.
+__device__ __forceinline__ uint64_t umma_desc_32b(uint32_t smem_addr_bytes) {
+  return static_cast<uint64_t>((smem_addr_bytes & 0x3ffffu) >> 4) | (1ull << 16) | (16ull << 32) | (1ull << 46) | (6ull << 61);
+}
+__device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z, unsigned long long pol) {
+  asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4, %5}], [%2], %6;"
+               :: "r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z), "l"(pol) : "memory");
+}
 __device__ __forceinline__ void umma_f16_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
@@ -184,7 +345,10 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
       : "r"(taddr) : "memory");
 }
 
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LMH_NT, 1) lm_head_kernel(const __grid_constant__ LmHeadArgs A) {
+// ADAPT: with D's adapters (D is null otherwise). It is then launched as a dependent of the kernel that makes h, with x and w there
+// before, and the products over K go on without waiting for it.
+template <bool ADAPT>
+__device__ __forceinline__ void lm_head_run(const LmHeadArgs& A, const LmAdaptArgs* D) {
   extern __shared__ __align__(16) unsigned char lmh_dyn[];
   __shared__ __align__(8) unsigned long long full_bar[LMH_MAX_STAGES], empty_bar[LMH_MAX_STAGES], acc_full[2], acc_empty[2];
   __shared__ uint32_t tmem_base_s;
@@ -246,6 +410,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LMH_NT, 1) lm_head_k
           for (int u = 0; u < subs; u++) tma_load_2d_pair(sx + u * x_bytes, &A.map_x, bar, (kc * LMH_SUB + u) * LMH_BK, xb, pol_x);
           if (++stage == static_cast<uint32_t>(nst)) { stage = 0; phase ^= 1u; }
         }
+        if constexpr (ADAPT) {
+          pdl_wait();
+          const int g = it.b0 / A.item_n, hrow = it.b0 - g * A.item_n + static_cast<int>(rank) * (it.n >> 1);
+          const int32_t* rec = D->groups + static_cast<int64_t>(g) * (LMA_HDR + A.item_n);
+          const int nu = ok ? rec[0] * D->units : 0;
+          for (int u0 = 0; u0 < nu; u0 += LMA_STAGE) {
+            if (!mbar_wait(smem_addr(&empty_bar[stage]), phase ^ 1u, abort_flag)) { ok = false; break; }
+            const uint32_t own = smem_addr(&full_bar[stage]), bar = map_rank(own, 0);
+            const uint32_t sw = ring + stage * stage_bytes, sx = sw + LMH_SUB * LMH_W_BYTES, hb = static_cast<uint32_t>(A.box_n) * 32;
+            const int here = min(LMA_STAGE, nu - u0);
+            if (rank == 0) mbar_expect_tx(own, 2 * here * (static_cast<uint32_t>(A.cta_v) * 32 + 2 * hb));
+            for (int u = 0; u < here; u++) {
+              const int slot = (u0 + u) / D->units, ru = (u0 + u) - slot * D->units;
+              tma_load_3d_pair(sw + u * (LMH_CTA_V * 32), &D->map_b, bar, ru * LMA_UNIT, v0, rec[LMA_HDR + slot], pol_w);
+              for (int piece = 0; piece < 2; piece++)
+                tma_load_2d_pair(sx + (2 * u + piece) * hb, &D->map_h, bar, 0, static_cast<int>(lma_h_row(*D, A.item_n, g, u0 + u, piece, hrow)), pol_x);
+            }
+            if (++stage == static_cast<uint32_t>(nst)) { stage = 0; phase ^= 1u; }
+          }
+        }
       }
     }
   } else if (warp == 1) {
@@ -270,6 +454,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LMH_NT, 1) lm_head_k
           }
           umma_commit_pair(smem_addr(&empty_bar[stage]));               // the stage is free once these MMAs have read it
           if (++stage == static_cast<uint32_t>(nst)) { stage = 0; phase ^= 1u; }
+        }
+        if constexpr (ADAPT) {
+          pdl_wait();
+          const int nu = ok ? D->groups[static_cast<int64_t>(plan.at(i).b0 / A.item_n) * (LMA_HDR + A.item_n)] * D->units : 0;
+          for (int u0 = 0; u0 < nu; u0 += LMA_STAGE) {
+            if (!mbar_wait(smem_addr(&full_bar[stage]), phase, abort_flag)) { ok = false; break; }
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint32_t sw = ring + stage * stage_bytes, sx = sw + LMH_SUB * LMH_W_BYTES, hb = static_cast<uint32_t>(A.box_n) * 32;
+            const int here = min(LMA_STAGE, nu - u0);
+            for (int u = 0; u < here; u++) {
+              for (int piece = 0; piece < 2; piece++)
+                umma_f16_pair(d_tmem, umma_desc_32b(sw + u * (LMH_CTA_V * 32)), umma_desc_32b(sx + (2 * u + piece) * hb), idesc, 1u);
+            }
+            umma_commit_pair(smem_addr(&empty_bar[stage]));
+            if (++stage == static_cast<uint32_t>(nst)) { stage = 0; phase ^= 1u; }
+          }
         }
         if (ok) umma_commit_pair(smem_addr(&acc_full[acc]));            // the accumulator is complete
         if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
@@ -299,6 +499,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LMH_NT, 1) lm_head_k
     if (A.chained) pdl_wait();                                          // the thresholds; tiles and MMAs are under way meanwhile
     for (int i = pair; i < plan.total && ok; i += npairs) {
       const LmhItem it = plan.at(i);
+      bool adapted = false;
+      if constexpr (ADAPT) adapted = D->groups[static_cast<int64_t>(it.b0 / A.item_n) * (LMA_HDR + A.item_n)] > 0;
       if (!mbar_wait(smem_addr(&acc_full[acc]), acc_phase, abort_flag)) { ok = false; break; }
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const int in_tile = static_cast<int>(rank) * A.cta_v + q * 32 + lane;
@@ -311,6 +513,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LMH_NT, 1) lm_head_k
         tmem_ld32(tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * LMH_MAX_N + c, r);
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
         const int b0 = it.b0 + c, nb = min(32, A.B - b0);              // batch rows of these columns (uniform)
+        if constexpr (ADAPT) {
+          if (adapted) {
+            uint32_t bad = 0u;
+#pragma unroll
+            for (int j = 0; j < 32; j++) bad |= (__uint_as_float(r[j]) != __uint_as_float(r[j])) ? 1u << j : 0u;
+            if (bad != 0u && live) {
+#pragma unroll 1
+              for (int j = 0; j < nb; j++) {
+                if (!((bad >> j) & 1u) || D->row_nan[b0 + j]) continue;
+                const uint32_t y = __float_as_uint(lma_logit(*D, A.K, A.item_n, b0 + j, v));
+#pragma unroll
+                for (int jj = 0; jj < 32; jj++) r[jj] = (j == jj) ? y : r[jj];
+              }
+            }
+            __syncwarp();
+          }
+        }
         if (A.out_logits && live) {
           float* dst = A.out_logits + static_cast<int64_t>(b0) * A.ld_out + ocol;
           if (nb == 32) {
@@ -385,6 +604,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LMH_NT, 1) lm_head_k
   }
 }
 
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LMH_NT, 1) lm_head_kernel(const __grid_constant__ LmHeadArgs A) {
+  lm_head_run<false>(A, nullptr);
+}
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LMH_NT, 1) lm_head_adapters_kernel(const __grid_constant__ LmHeadArgs A, const __grid_constant__ LmAdaptArgs D) {
+  lm_head_run<true>(A, &D);
+}
 
 // ---- fused sampling on top of the projection (greedy and top-k rows) --------------------------------
 //

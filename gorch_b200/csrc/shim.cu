@@ -671,6 +671,22 @@ int make_bf16_map(CUtensorMap* map, const void* base, int64_t rows, int64_t K, i
   return GORCH_CUDA_OK;
 }
 
+// Tensor map of rows of bf16 for the 32-byte swizzle: boxes of 16 columns x box_rows rows; a third dimension of `deep` matrices when above 0.
+int make_unit_map(CUtensorMap* map, const void* base, int64_t cols, int64_t rows, int64_t ld, int64_t deep, int64_t deep_stride, int box_rows, char** errOut) {
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(deep)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(ld) * 2, static_cast<cuuint64_t>(deep_stride) * 2};
+  const cuuint32_t box[3] = {static_cast<cuuint32_t>(gs::LMA_UNIT), static_cast<cuuint32_t>(box_rows), 1};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = g_encode_tiled(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, deep > 0 ? 3 : 2, const_cast<void*>(base), dims, strides, box, estr,
+                                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_32B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_err(errOut, "gorch_cuda: cuTensorMapEncodeTiled failed with code %d", static_cast<int>(r));
+    return GORCH_CUDA_ERR_CUDA;
+  }
+  return GORCH_CUDA_OK;
+}
+
 int check_lm_head(Ctx* c, const void* x, const void* w, int64_t B, int64_t V, int64_t K, int64_t ldx, int64_t ldw, char** errOut) {
   if (B < 0 || V < 1 || K < gs::LMH_BK || (K % gs::LMH_BK) != 0 || ldx < K || ldw < K) {
     set_err(errOut, "gorch_cuda: LM head needs B >= 0, V >= 1 and K a multiple of %d (got B=%lld V=%lld K=%lld)", gs::LMH_BK,
@@ -716,8 +732,8 @@ int lm_head_args(const Ctx* c, gs::LmHeadArgs& a, const void* x, int64_t ldx, co
 
 // One launch of lm_head_kernel over the vocabulary tiles tile0 + i * step, i < ntile. chained: behind the kernel that fills the
 // thresholds. dependent: it may start beside the end of the kernel before it (the first one of a chain does not: the
-// chain's second projection reads x and w without waiting for what came before the chain).
-int launch_lm_head(Ctx* c, gs::LmHeadArgs& a, char** errOut, bool dependent, bool chained = false) {
+// chain's second projection reads x and w without waiting for what came before the chain). d: with these adapters.
+int launch_lm_head(Ctx* c, gs::LmHeadArgs& a, char** errOut, bool dependent, bool chained = false, const gs::LmAdaptArgs* d = nullptr) {
   const int64_t ntile_total = (static_cast<int64_t>(a.V) + 2 * a.cta_v - 1) / (2 * a.cta_v);
   if (a.ntile < 1 || a.tile0 + static_cast<int64_t>(a.ntile - 1) * a.tile_step >= ntile_total) {
     set_err(errOut, "gorch_cuda: LM head tile range outside the vocabulary");
@@ -728,8 +744,9 @@ int launch_lm_head(Ctx* c, gs::LmHeadArgs& a, char** errOut, bool dependent, boo
   if (npairs > most) npairs = most;
   a.status = c->host_words;
   a.chained = chained ? 1 : 0;
-  a.clear_status = chained ? 0 : 1;
-  CUDA_TRY(launch(c, gs::lm_head_kernel, static_cast<unsigned>(2 * npairs), gs::LMH_NT, gs::LMH_DYN_BYTES, dependent, a), errOut);
+  a.clear_status = chained && !d ? 0 : 1;
+  if (d) CUDA_TRY(launch(c, gs::lm_head_adapters_kernel, static_cast<unsigned>(2 * npairs), gs::LMH_NT, gs::LMH_DYN_BYTES, dependent, a, *d), errOut);
+  else CUDA_TRY(launch(c, gs::lm_head_kernel, static_cast<unsigned>(2 * npairs), gs::LMH_NT, gs::LMH_DYN_BYTES, dependent, a), errOut);
   c->counters.kernel_launches += 1;
   return GORCH_CUDA_OK;
 }
@@ -847,6 +864,7 @@ GorchCudaCtxRef gorch_cuda_create_ctx(int device, char** errOut) {
   if ((e = cudaFuncSetAttribute(gs::w1024::wide_rows_kernel<float>, cudaFuncAttributeMaxDynamicSharedMemorySize, gs::w1024::W_DYN_BYTES)) != cudaSuccess) return fail("cudaFuncSetAttribute", e);
   if ((e = cudaFuncSetAttribute(gs::w1024::wide_rows_kernel<uint16_t>, cudaFuncAttributeMaxDynamicSharedMemorySize, gs::w1024::W_DYN_BYTES)) != cudaSuccess) return fail("cudaFuncSetAttribute", e);
   if ((e = cudaFuncSetAttribute(gs::lm_head_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, gs::LMH_DYN_BYTES)) != cudaSuccess) return fail("cudaFuncSetAttribute", e);
+  if ((e = cudaFuncSetAttribute(gs::lm_head_adapters_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, gs::LMH_DYN_BYTES)) != cudaSuccess) return fail("cudaFuncSetAttribute", e);
   if ((e = cudaFuncSetAttribute(gs::lmh_finish_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, gs::LMH_F_DYN_BYTES)) != cudaSuccess) return fail("cudaFuncSetAttribute", e);
   if ((e = cudaFuncSetAttribute(gs::row_softmax_kernel<float>, cudaFuncAttributeMaxDynamicSharedMemorySize, gs::RS_DYN_BYTES)) != cudaSuccess) return fail("cudaFuncSetAttribute", e);
   if ((e = cudaFuncSetAttribute(gs::row_softmax_kernel<uint16_t>, cudaFuncAttributeMaxDynamicSharedMemorySize, gs::RS_DYN_BYTES)) != cudaSuccess) return fail("cudaFuncSetAttribute", e);
@@ -1911,6 +1929,98 @@ int gorch_cuda_lm_head_logits_dev(GorchCudaCtxRef ctx, const void* x, int64_t ld
   a.tile0 = 0; a.tile_step = 1; a.ntile = static_cast<int32_t>((V + 2 * a.cta_v - 1) / (2 * a.cta_v));
   a.out_logits = out_logits; a.ld_out = ld_out; a.compact = 0;
   return launch_lm_head(c, a, errOut, true);
+}
+
+// The workspace of a call with adapters: [group records | NaN marks of the rows | h], for groups of item_n batch rows.
+struct AdapterSpace { int64_t item_n, groups, units, max_units, off_nan, off_h, bytes; };
+static AdapterSpace adapter_space(int64_t B, const GorchAdapters* ad) {
+  AdapterSpace s;
+  s.item_n = B >= gs::LMH_MAX_N ? gs::LMH_MAX_N : (B + 31) & ~31ll;
+  s.groups = (B + s.item_n - 1) / s.item_n;
+  s.units = (ad->rank + gs::LMA_UNIT - 1) / gs::LMA_UNIT;
+  s.max_units = (ad->n < s.item_n ? ad->n : s.item_n) * s.units;
+  s.off_nan = (s.groups * (gs::LMA_HDR + s.item_n) * 4 + 255) & ~255ll;
+  s.off_h = (s.off_nan + B * 4 + 255) & ~255ll;
+  s.bytes = s.off_h + s.groups * s.max_units * 2 * s.item_n * gs::LMA_UNIT * 2;
+  return s;
+}
+
+static int check_adapters(const GorchAdapters* ad, int64_t V, int64_t K, char** errOut) {
+  if (!ad) { set_err(errOut, "gorch_cuda: null adapters record"); return GORCH_CUDA_ERR_BAD_ARG; }
+  if (ad->n < 1 || ad->rank < 1) { set_err(errOut, "gorch_cuda: adapters need n >= 1 and rank >= 1, got %lld and %lld", (long long)ad->n, (long long)ad->rank); return GORCH_CUDA_ERR_BAD_ARG; }
+  if (ad->rank > gs::LMA_MAX_RANK || ad->n > 0x7fffffffll) { set_err(errOut, "gorch_cuda: adapter rank beyond %d or more than 2^31 adapters", gs::LMA_MAX_RANK); return GORCH_CUDA_ERR_LIMIT; }
+  if (V == 0) return GORCH_CUDA_OK;                          // (the workspace's size alone)
+  if (!ad->a || !ad->b) { set_err(errOut, "gorch_cuda: null pointer argument"); return GORCH_CUDA_ERR_BAD_ARG; }
+  const int64_t a_all = (ad->rank - 1) * ad->a_pitch + K, b_all = (V - 1) * ad->b_pitch + ad->rank;
+  if (ad->a_pitch < K || ad->b_pitch < ad->rank || (ad->n > 1 && (ad->a_stride < a_all || ad->b_stride < b_all))) {
+    set_err(errOut, "gorch_cuda: adapters' pitches and strides must not make rows overlap");
+    return GORCH_CUDA_ERR_BAD_ARG;
+  }
+  if ((reinterpret_cast<uintptr_t>(ad->a) & 15u) || (reinterpret_cast<uintptr_t>(ad->b) & 15u) || (reinterpret_cast<uintptr_t>(ad->scales) & 3u) ||
+      (ad->a_pitch & 7) || (ad->b_pitch & 7) || (ad->n > 1 && ((ad->a_stride & 7) || (ad->b_stride & 7)))) {
+    set_err(errOut, "gorch_cuda: adapters must be 16-byte aligned with pitches and strides that are multiples of 16 bytes");
+    return GORCH_CUDA_ERR_BAD_ARG;
+  }
+  return GORCH_CUDA_OK;
+}
+
+int gorch_cuda_lm_head_adapters_workspace(int64_t B, const GorchAdapters* adapters, uint64_t* bytes, char** errOut) {
+  if (!bytes) { set_err(errOut, "gorch_cuda: null pointer argument"); return GORCH_CUDA_ERR_BAD_ARG; }
+  const int rc = check_adapters(adapters, 0, 0, errOut);
+  if (rc) return rc;
+  if (B < 0) { set_err(errOut, "gorch_cuda: bad batch size %lld", (long long)B); return GORCH_CUDA_ERR_BAD_ARG; }
+  if (B > 0x7fffffffll) { set_err(errOut, "gorch_cuda: batch beyond 31 bits"); return GORCH_CUDA_ERR_LIMIT; }
+  *bytes = B == 0 ? 0 : static_cast<uint64_t>(adapter_space(B, adapters).bytes);
+  return GORCH_CUDA_OK;
+}
+
+int gorch_cuda_lm_head_adapters_dev(GorchCudaCtxRef ctx, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t B, int64_t V, int64_t K,
+                                    const GorchAdapters* adapters, const int32_t* row_adapter, void* workspace, uint64_t workspace_bytes,
+                                    float* out_logits, int64_t ld_out, char** errOut) {
+  Ctx* c = static_cast<Ctx*>(ctx);
+  if (!c) { set_err(errOut, "gorch_cuda: null context"); return GORCH_CUDA_ERR_BAD_ARG; }
+  int rc = check_lm_head(c, x, w, B, V, K, ldx, ldw, errOut);
+  if (rc || (rc = check_adapters(adapters, V, K, errOut))) return rc;
+  if (B == 0) return GORCH_CUDA_OK;
+  if (!out_logits || ld_out < V) { set_err(errOut, "gorch_cuda: LM head output missing or its pitch below V"); return GORCH_CUDA_ERR_BAD_ARG; }
+  if (!row_adapter || !workspace) { set_err(errOut, "gorch_cuda: null pointer argument"); return GORCH_CUDA_ERR_BAD_ARG; }
+  if ((reinterpret_cast<uintptr_t>(row_adapter) & 3u) || (reinterpret_cast<uintptr_t>(out_logits) & 3u) || (reinterpret_cast<uintptr_t>(workspace) & 255u)) {
+    set_err(errOut, "gorch_cuda: row_adapter and the output must be 4-byte aligned, the workspace 256-byte aligned");
+    return GORCH_CUDA_ERR_BAD_ARG;
+  }
+  const AdapterSpace sp = adapter_space(B, adapters);
+  if (workspace_bytes < static_cast<uint64_t>(sp.bytes)) {
+    set_err(errOut, "gorch_cuda: workspace of %llu bytes, %lld needed", (unsigned long long)workspace_bytes, (long long)sp.bytes);
+    return GORCH_CUDA_ERR_BAD_ARG;
+  }
+  const int64_t h_rows = sp.groups * sp.max_units * 2 * sp.item_n;
+  if (h_rows > 0x7fffffffll) { set_err(errOut, "gorch_cuda: more adapters and batch rows than 31 bits of workspace rows hold"); return GORCH_CUDA_ERR_LIMIT; }
+  CUDA_TRY(cudaSetDevice(c->device), errOut);
+  if ((rc = load_encode_tiled(errOut))) return rc;
+  gs::LmHeadArgs a;
+  if ((rc = lm_head_args(c, a, x, ldx, w, ldw, B, V, K, true, errOut))) return rc;
+  a.tile0 = 0; a.tile_step = 1; a.ntile = static_cast<int32_t>((V + 2 * a.cta_v - 1) / (2 * a.cta_v));
+  a.out_logits = out_logits; a.ld_out = ld_out; a.compact = 0;
+  gs::LmAdaptArgs d;
+  memset(&d, 0, sizeof d);
+  d.x = static_cast<const uint16_t*>(x); d.w = static_cast<const uint16_t*>(w); d.ldx = ldx; d.ldw = ldw;
+  d.a = static_cast<const uint16_t*>(adapters->a); d.b = static_cast<const uint16_t*>(adapters->b);
+  d.a_pitch = adapters->a_pitch; d.b_pitch = adapters->b_pitch;
+  d.a_stride = adapters->n > 1 ? adapters->a_stride : 0;
+  d.b_stride = adapters->n > 1 ? adapters->b_stride : V * adapters->b_pitch;
+  d.scales = adapters->scales; d.row_adapter = row_adapter;
+  d.n = static_cast<int32_t>(adapters->n); d.rank = static_cast<int32_t>(adapters->rank);
+  d.units = static_cast<int32_t>(sp.units); d.max_units = static_cast<int32_t>(sp.max_units);
+  unsigned char* base = static_cast<unsigned char*>(workspace);
+  d.groups = reinterpret_cast<int32_t*>(base);
+  d.row_nan = reinterpret_cast<int32_t*>(base + sp.off_nan);
+  d.h = reinterpret_cast<uint16_t*>(base + sp.off_h);
+  if ((rc = make_unit_map(&d.map_b, adapters->b, adapters->rank, V, adapters->b_pitch, adapters->n, d.b_stride, a.cta_v, errOut))) return rc;
+  if ((rc = make_unit_map(&d.map_h, d.h, gs::LMA_UNIT, h_rows, gs::LMA_UNIT, 0, 0, a.box_n, errOut))) return rc;
+  // (not a dependent: what it has waited for, the projection behind it reads without waiting)
+  CUDA_TRY(launch(c, gs::lm_adapters_kernel, static_cast<unsigned>(B), gs::LMA_NT, 0, false, d, a.B, a.K, a.item_n), errOut);
+  c->counters.kernel_launches += 1;
+  return launch_lm_head(c, a, errOut, true, true, &d);
 }
 
 int gorch_cuda_lm_head_sample_dev(GorchCudaCtxRef ctx, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t B,

@@ -410,6 +410,23 @@ class CudaSampler:
         rc = self._lib.gorch_cuda_lm_head_logits_dev(self._ctx, x_ptr, ldx, w_ptr, ldw, B, V, K, out_ptr, ld_out, C.byref(err))
         _check(self._lib, rc, err)
 
+    def lm_head_adapters_workspace(self, B: int, adapters) -> int:
+        """gorch_cuda_lm_head_adapters_workspace: bytes of device memory that lm_head_adapters_ptrs needs for B rows."""
+        n, err = C.c_uint64(0), C.c_void_p()
+        rc = self._lib.gorch_cuda_lm_head_adapters_workspace(B, C.byref(adapters) if adapters is not None else None, C.byref(n), C.byref(err))
+        _check(self._lib, rc, err)
+        return int(n.value)
+
+    def lm_head_adapters_ptrs(self, x_ptr: int, ldx: int, w_ptr: int, ldw: int, B: int, V: int, K: int, adapters, row_adapter_ptr: int,
+                              workspace_ptr: int, workspace_bytes: int, out_ptr: int, ld_out: int) -> None:
+        """gorch_cuda_lm_head_adapters_dev: lm_head_logits_ptrs plus each row's low-rank adapter (`adapters`: a _lib.Adapters
+        record; row_adapter [B] int32, -1 for none); device pointers."""
+        err = C.c_void_p()
+        rc = self._lib.gorch_cuda_lm_head_adapters_dev(self._ctx, x_ptr, ldx, w_ptr, ldw, B, V, K,
+                                                       C.byref(adapters) if adapters is not None else None, row_adapter_ptr,
+                                                       workspace_ptr, workspace_bytes, out_ptr, ld_out, C.byref(err))
+        _check(self._lib, rc, err)
+
     def lm_head_sample_ptrs(self, x_ptr: int, ldx: int, w_ptr: int, ldw: int, B: int, V: int, K: int, fuse_top_k: int,
                             cfgs_ptr: int, uniforms_ptr: int, ids_ptr: int, flags_ptr: int | None = None) -> None:
         """gorch_cuda_lm_head_sample_dev: projection + sampling in one call; device pointers."""

@@ -443,6 +443,29 @@ int gorch_cuda_lm_head_logits_dev(GorchCudaCtxRef ctx, const void* x, int64_t ld
                                   int64_t B, int64_t V, int64_t K, float* out_logits, int64_t ld_out,
                                   char** errOut);
 int gorch_cuda_lm_head_status(GorchCudaCtxRef ctx, uint32_t* status, char** errOut);
+/* The projection with a low-rank adapter of its own for each row (no counterpart in the reference's decode path, whose
+ * projection is the plain MatMulTransB above):
+ *   logits[b, v] = sum_k x[b, k] w[v, k] + scales[i] sum_r b[i, v, r] (sum_k a[i, r, k] x[b, k]),   i = row_adapter[b]
+ * in one pass over the weights, whatever adapters the rows of a batch have; a row whose row_adapter lies
+ * outside [0, n) (-1) gets the projection alone. a and b are bf16, sums are f32, and the inner product with a is handed on in two
+ * bf16 (it loses 2^-16 at most). What one row's adapter holds does not reach other rows, infinities and NaN
+ * included. Operands as for gorch_cuda_lm_head_logits_dev; a and b 16-byte aligned, pitches and strides multiples of 8
+ * elements; rank 1 .. 256. The workspace (device memory of the size that gorch_cuda_lm_head_adapters_workspace
+ * gives, 256-byte aligned) is the call's while it runs: calls that may overlap, captured ones among them,
+ * each need their own. Asynchronous; gorch_cuda_lm_head_status covers it. */
+typedef struct {
+  const void* a;        /* [n][rank][K]: row pitch a_pitch, from one adapter to the next a_stride elements */
+  int64_t a_pitch, a_stride;
+  const void* b;        /* [n][V][rank]: row pitch b_pitch, from one adapter to the next b_stride elements */
+  int64_t b_pitch, b_stride;
+  const float* scales;  /* [n], or NULL: 1 */
+  int64_t n, rank;
+} GorchAdapters;
+int gorch_cuda_lm_head_adapters_workspace(int64_t B, const GorchAdapters* adapters, uint64_t* bytes, char** errOut);
+int gorch_cuda_lm_head_adapters_dev(GorchCudaCtxRef ctx, const void* x, int64_t ldx, const void* w, int64_t ldw,
+                                    int64_t B, int64_t V, int64_t K, const GorchAdapters* adapters,
+                                    const int32_t* row_adapter, void* workspace, uint64_t workspace_bytes,
+                                    float* out_logits, int64_t ld_out, char** errOut);
 /* The projection and the sampling step in one call: out_ids[b] = the token sampled from row b of
  * x @ w^T under cfgs[b] with uniforms[b], as gorch_cuda_sample_dev would return on the materialised
  * logits. fuse_top_k in 1..256: the batch's largest top_k; rows with temperature 0 or 0 < top_k <=
