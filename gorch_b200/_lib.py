@@ -120,7 +120,7 @@ def load() -> C.CDLL:
         "gorch_cuda_lm_head_logits_dev": (i32, [p, p, i64, p, i64, i64, i64, i64, p, i64, err]),
         "gorch_cuda_lm_head_status": (i32, [p, C.POINTER(C.c_uint32), err]),
         "gorch_cuda_lm_head_sample_dev": (i32, [p, p, i64, p, i64, i64, i64, i64, i32, p, p, p, p, err]),
-        "gorch_cuda_lm_head_adapters_workspace": (i32, [i64, C.POINTER(Adapters), C.POINTER(C.c_uint64), err]),
+        "gorch_cuda_lm_head_adapters_workspace": (i32, [i64, i64, C.POINTER(Adapters), C.POINTER(C.c_uint64), err]),
         "gorch_cuda_lm_head_adapters_dev": (i32, [p, p, i64, p, i64, i64, i64, i64, C.POINTER(Adapters), p, p, C.c_uint64, p, i64, err]),
         "gorch_cuda_topk_dev": (i32, [p, p, i32, i64, i64, i64, i64, p, p, p, err]),
         "gorch_cuda_multinomial_dev": (i32, [p, p, i64, i64, i64, p, p, p, err]),

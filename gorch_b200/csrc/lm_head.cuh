@@ -93,78 +93,147 @@ struct LmHeadArgs {
 
 // ---- low-rank adapters beside the projection -----------------------------------------------------------
 // logits[b, v] += h[b] . b[a][v], h[b] = scale[a] * (a[a] x[b]), for the adapter a that row b has (none: no term). For the tensor pipe
-// these are further columns of K: for every adapter that a group of item_n batch rows uses, its b [V, rank] on the w side, and
-// on the x side h in the rows that use it and 0 in the others. So the products of an item go on, after K, over the group's
-// adapters in units of LMA_UNIT columns of the rank, LMA_STAGE of them in a stage of the ring (32-byte rows, 32-byte swizzle; what a
-// rank leaves of a unit is filled with zeros by the copy). The rows need no order, every adapter's b passes once per
-// batch group, and the epilogue's results are complete. h goes in as two bf16, the rounded value and what the rounding left (2^-16 of
-// it is lost at most, about what the f32 sums over K lose), each multiplied with the same tile of b: one bf16 would put 2^-9 of
-// the adapter's term on logits that are f32.
-// 0 times an Inf or NaN in an adapter's b is NaN, in rows that do not use that adapter too (and the two parts of h may disagree about an
-// Inf in the row's own): where a group has adapters, the epilogue works a NaN out again from the row's own operands, unless x holds one.
+// these are further columns of K. The batch rows are taken in the order of their adapters (x is copied in that order, and the
+// epilogue writes to the rows' own places), so that in a group of item_n of them an adapter's rows are a run. After K the
+// products of an item go on over its runs, in units of LMA_UNIT columns of the rank: the adapter's b [V, rank] on the w side, h
+// on the x side, over the multiple of 32 batch rows that holds the run, with zeros in the rows around it. LMA_STAGE units share a
+// stage of the ring (32-byte rows, 32-byte swizzle; what a rank leaves of a unit is filled with zeros by the copy). Four warps of
+// their own ask for a stage's units, one each, once the producer has found the stage free and announced its bytes: asking for
+// all of them took one thread 0.4 us a unit (256 rows with 32 adapters of rank 32: 355 us, AAA so; the projection alone 96).
+// (cp.async instead of TMA, 16 bytes a lane and a warp per stage: 401.)
+// So an adapter's b passes once per group, its products cost what its rows cost, rounded up to 32 (with every unit over all
+// rows of the item, 256 x 1,024 x 151,936 with 32 adapters of rank 32 took 290 us), and the epilogue's results are complete.
+// h goes in as two bf16, the rounded value and what the rounding left, each multiplied with the same tile of b: one bf16 would put
+// 2^-8 of the adapter's term on logits that are f32, two lose 2^-16 of it at most (the sums over K = 1,024, which the tensor pipe
+// cuts off rather than rounds, are off by 1.0e-6 of the logits' size by themselves, with the adapters 1.3e-6).
+// 0 times an Inf or NaN in an adapter's b is NaN, in the rows around its run too (and the two parts of h may disagree about an Inf in the
+// row's own): where a group has adapters, the epilogue works a NaN out again from the row's own operands, unless x holds one.
 constexpr int LMA_UNIT = 16;             // columns of the rank in a unit: K of one MMA, 32 bytes
-constexpr int LMA_STAGE = 4;             // units in a stage
+constexpr int LMA_STAGE = 4;             // units in a stage, and warps of a CTA that ask for them: one for each of a stage's units
+constexpr int LMA_RUN_NT = LMH_NT + 32 * LMA_STAGE;
+constexpr int LMA_RING_BYTES = 200 * 1024, LMA_DYN_BYTES = LMA_RING_BYTES + 1024;
 constexpr int LMA_MAX_RANK = 256;
-constexpr int LMA_NT = 256;              // of the kernel that makes h
-constexpr int LMA_HDR = 4;               // words of a group's record ahead of its adapters: the first one says how many
+constexpr int LMA_NT = 256;              // of the kernels ahead of the projection
+constexpr int LMA_BOX = 16;              // batch rows of h that one TMA load brings
 static_assert(LMA_STAGE * 2 * 32 <= LMH_SUB * LMH_BK * 2 && LMA_STAGE * LMH_CTA_V * 32 <= LMH_SUB * LMH_W_BYTES, "a stage holds its units");
+static_assert(LMA_NT >= LMH_MAX_N, "a thread per batch row of a group");
 
+struct LmaRun { int32_t adapter, n0, n1, pad; };   // of a group: its rows n0 .. n1 - 1, multiples of 32, hold the adapter's
 struct LmAdaptArgs {
   CUtensorMap map_b;       // b [n, V, rank] bf16, box 16 x cta_v, 32-byte swizzle
-  CUtensorMap map_h;       // h [group][unit][2][item_n] rows of 16 bf16, box 16 x box_n, 32-byte swizzle
+  CUtensorMap map_h;       // h [group][unit][2][item_n] rows of 16 bf16, box 16 x LMA_BOX, 32-byte swizzle
   const uint16_t *x, *w, *a, *b;
   int64_t ldx, ldw, a_pitch, a_stride, b_pitch, b_stride;   // in elements
   const float* scales;     // [n] or null: 1
   const int32_t* row_adapter;   // [B]; outside [0, n): none
   int32_t n, rank, units;  // adapters, their rank, units of one
-  int32_t max_units;       // of a group
-  int32_t* groups;         // [group][LMA_HDR + item_n]
-  int32_t* row_nan;        // [B]
+  int32_t max_runs;        // of a group
+  int32_t B, K, item_n;
+  // the workspace
+  int32_t* nruns;          // [group]
+  LmaRun* runs;            // [group][max_runs]
+  int32_t* order;          // [B] the row at each place of the order
+  int32_t* sorted;         // [B] its adapter, -1: none
+  int32_t* row_nan;        // [B] whether its x holds a NaN
+  uint16_t* xs;            // [B, K] x in that order
   uint16_t* h;
 };
-__host__ __device__ inline int64_t lma_h_row(const LmAdaptArgs& D, int item_n, int group, int unit, int piece, int row) {
-  return ((static_cast<int64_t>(group) * D.max_units + unit) * 2 + piece) * item_n + row;
+__device__ __forceinline__ int64_t lma_h_row(const LmAdaptArgs& D, int group, int unit, int piece, int row) {
+  return ((static_cast<int64_t>(group) * D.max_runs * D.units + unit) * 2 + piece) * D.item_n + row;
 }
 
 __device__ __forceinline__ float bf16_lo(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
 
-// A CTA per batch row: which adapters its group uses (in the order of their first rows), and its h for all of them.
-__global__ void __launch_bounds__(LMA_NT) lm_adapters_kernel(const __grid_constant__ LmAdaptArgs D, const int32_t B, const int32_t K, const int32_t item_n) {
-  __shared__ __align__(16) int s_ad[LMA_NT];
-  __shared__ int s_first[LMA_NT / 32], s_mine;
+// The place of row b in the order of (adapter, row), rows without one last. All of the CTA's threads; keys: 4 * LMA_NT words.
+__device__ __forceinline__ int lma_place(const LmAdaptArgs& D, int b, int key, int* keys, int tid) {
+  int place = 0;
+  for (int j0 = 0; j0 < D.B; j0 += 4 * LMA_NT) {
+    __syncthreads();
+    for (int j = tid; j < 4 * LMA_NT; j += LMA_NT) {
+      const int a = j0 + j < D.B ? D.row_adapter[j0 + j] : 0;
+      keys[j] = j0 + j < D.B ? ((a < 0 || a >= D.n) ? D.n : a) : 0x7fffffff;
+    }
+    __syncthreads();
+    const int lim = min(4 * LMA_NT, D.B - j0);
+#pragma unroll 4
+    for (int j = 0; j < lim; j += 4) {
+      const int4 o = *reinterpret_cast<const int4*>(&keys[j]);
+      const int at = j0 + j;
+      place += (o.x < key || (o.x == key && at < b)) + (o.y < key || (o.y == key && at + 1 < b)) + (o.z < key || (o.z == key && at + 2 < b)) +
+               (o.w < key || (o.w == key && at + 3 < b));
+    }
+  }
+  return place;
+}
+__global__ void __launch_bounds__(LMA_NT) lm_adapters_order_kernel(const __grid_constant__ LmAdaptArgs D) {
+  __shared__ __align__(16) int keys[4 * LMA_NT];
+  const int tid = threadIdx.x, b = blockIdx.x * LMA_NT + tid;
+  int a = b < D.B ? D.row_adapter[b] : -1;
+  if (a < 0 || a >= D.n) a = -1;
+  const int place = lma_place(D, b, a < 0 ? D.n : a, keys, tid);
+  if (b < D.B) { D.order[place] = b; D.sorted[place] = a; }
+  pdl_launch();
+}
+
+// A CTA per place of the order: the runs of its group, its row of x, its h. A batch of one group is put in order here (ordered == 0).
+__global__ void __launch_bounds__(LMA_NT) lm_adapters_kernel(const __grid_constant__ LmAdaptArgs D, const int32_t ordered) {
+  __shared__ __align__(16) int keys[4 * LMA_NT];
+  __shared__ int s_ad[LMA_NT + 1], s_start[LMA_NT + 1], s_first[LMA_NT / 32], s_row, s_mine;
   __shared__ float s_h[LMA_MAX_RANK];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int b = blockIdx.x, g = b / item_n, g0 = g * item_n, rows = min(item_n, B - g0);
+  const int p = blockIdx.x, g = p / D.item_n, g0 = g * D.item_n, rows = min(D.item_n, D.B - g0);
   pdl_launch();
-  int a = (tid < rows) ? D.row_adapter[g0 + tid] : -1;
-  if (a < 0 || a >= D.n) a = -1;
-  s_ad[tid] = a;
+  if (ordered) {
+    pdl_wait();
+    s_ad[tid] = tid < rows ? D.sorted[g0 + tid] : -1;
+    if (tid == 0) s_row = D.order[p];
+  } else {
+    int a = tid < D.B ? D.row_adapter[tid] : -1;
+    if (a < 0 || a >= D.n) a = -1;
+    s_ad[tid] = -1;
+    const int place = lma_place(D, tid, a < 0 ? D.n : a, keys, tid);   // (its barriers come before the next line)
+    if (tid < D.B) {
+      s_ad[place] = a;
+      if (place == p) s_row = tid;
+      if (p == 0) { D.order[place] = tid; D.sorted[place] = a; }
+    }
+  }
   if (tid == 0) s_mine = -1;
   __syncthreads();
-  bool first = a >= 0;
-#pragma unroll 4
-  for (int j = 0; j < tid; j += 4) {
-    const int4 o = *reinterpret_cast<const int4*>(&s_ad[j]);
-    if (o.x == a || (o.y == a && j + 1 < tid) || (o.z == a && j + 2 < tid) || (o.w == a && j + 3 < tid)) first = false;
-  }
+  const int a = s_ad[tid];
+  const bool first = a >= 0 && (tid == 0 || s_ad[tid - 1] != a);
   const uint32_t votes = __ballot_sync(FULL, first);
   if (lane == 0) s_first[warp] = __popc(votes);
+  const int taught = __syncthreads_count(a >= 0);                    // rows with an adapter: the first ones
+  int run = __popc(votes & ((1u << lane) - 1u)), nruns = 0;
+  for (int w = 0; w < LMA_NT / 32; w++) { run += w < warp ? s_first[w] : 0; nruns += s_first[w]; }
+  if (first) s_start[run] = tid;
+  if (tid == 0) s_start[nruns] = taught;
   __syncthreads();
-  const int mine = s_ad[b - g0];
-  int slot = __popc(votes & ((1u << lane) - 1u)), nslots = 0;
-  for (int w = 0; w < LMA_NT / 32; w++) { slot += w < warp ? s_first[w] : 0; nslots += s_first[w]; }
-  if (first && a == mine) s_mine = slot;
-  int32_t* rec = D.groups + static_cast<int64_t>(g) * (LMA_HDR + item_n);
-  __syncthreads();                                                   // s_mine
-  if (b == g0) {
-    if (first) rec[LMA_HDR + slot] = a;
-    if (tid == 0) rec[0] = nslots;
+  const int mine = s_ad[p - g0], row = s_row;
+  if (tid < nruns) {
+    LmaRun r;
+    r.adapter = s_ad[s_start[tid]];
+    r.n0 = s_start[tid] & ~31;
+    r.n1 = (s_start[tid + 1] + 31) & ~31;
+    r.pad = 0;
+    if (p == g0) D.runs[static_cast<int64_t>(g) * D.max_runs + tid] = r;
+    if (r.adapter == mine) s_mine = tid;
   }
-  // h = scale * a x, a rank's row per warp
-  const uint4* x4 = reinterpret_cast<const uint4*>(D.x + b * D.ldx);
-  const int nk = K / 8;
+  if (p == g0 && tid == 0) D.nruns[g] = nruns;
+  // x in its place, and h = scale * a x, a rank's row per warp
+  const uint4* x4 = reinterpret_cast<const uint4*>(D.x + row * D.ldx);
+  uint4* xs4 = reinterpret_cast<uint4*>(D.xs + static_cast<int64_t>(p) * D.K);
+  const int nk = D.K / 8;
   bool nan = false;
+  for (int k = tid; k < nk; k += LMA_NT) {
+    const uint4 q = __ldg(x4 + k);
+    xs4[k] = q;
+    const uint32_t ws[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int c = 0; c < 4; c++) nan |= (ws[c] & 0x7fffu) > 0x7f80u || (ws[c] & 0x7fff0000u) > 0x7f800000u;
+  }
   if (mine >= 0) {
     const float scale = D.scales ? D.scales[mine] : 1.0f;
     for (int r = warp; r < D.rank; r += LMA_NT / 32) {
@@ -172,34 +241,27 @@ __global__ void __launch_bounds__(LMA_NT) lm_adapters_kernel(const __grid_consta
       float acc = 0.0f;
 #pragma unroll 4
       for (int k = lane; k < nk; k += 32) {
-        const uint4 p = __ldg(x4 + k), q = __ldg(a4 + k);
-        acc = fmaf(bf16_lo(p.x), bf16_lo(q.x), acc); acc = fmaf(bf16_hi(p.x), bf16_hi(q.x), acc);
-        acc = fmaf(bf16_lo(p.y), bf16_lo(q.y), acc); acc = fmaf(bf16_hi(p.y), bf16_hi(q.y), acc);
-        acc = fmaf(bf16_lo(p.z), bf16_lo(q.z), acc); acc = fmaf(bf16_hi(p.z), bf16_hi(q.z), acc);
-        acc = fmaf(bf16_lo(p.w), bf16_lo(q.w), acc); acc = fmaf(bf16_hi(p.w), bf16_hi(q.w), acc);
+        const uint4 q = __ldg(x4 + k), t = __ldg(a4 + k);
+        acc = fmaf(bf16_lo(q.x), bf16_lo(t.x), acc); acc = fmaf(bf16_hi(q.x), bf16_hi(t.x), acc);
+        acc = fmaf(bf16_lo(q.y), bf16_lo(t.y), acc); acc = fmaf(bf16_hi(q.y), bf16_hi(t.y), acc);
+        acc = fmaf(bf16_lo(q.z), bf16_lo(t.z), acc); acc = fmaf(bf16_hi(q.z), bf16_hi(t.z), acc);
+        acc = fmaf(bf16_lo(q.w), bf16_lo(t.w), acc); acc = fmaf(bf16_hi(q.w), bf16_hi(t.w), acc);
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(FULL, acc, o);
       if (lane == 0) s_h[r] = acc * scale;
     }
   }
-  for (int k = tid; k < nk; k += LMA_NT) {
-    const uint4 p = __ldg(x4 + k);
-    const float t = (bf16_lo(p.x) * 0.0f + bf16_hi(p.x) * 0.0f) + (bf16_lo(p.y) * 0.0f + bf16_hi(p.y) * 0.0f) + (bf16_lo(p.z) * 0.0f + bf16_hi(p.z) * 0.0f) +
-                    (bf16_lo(p.w) * 0.0f + bf16_hi(p.w) * 0.0f);
-    if (t != t) {                                                    // a NaN or an infinity
-      const uint32_t ws[4] = {p.x, p.y, p.z, p.w};
-      for (int c = 0; c < 4; c++) nan |= bf16_lo(ws[c]) != bf16_lo(ws[c]) || bf16_hi(ws[c]) != bf16_hi(ws[c]);
-    }
-  }
-  const int any = __syncthreads_or(nan);                             // (and s_h is there)
-  if (tid == 0) D.row_nan[b] = any;
-  // 16 bytes at a time: of every unit's row of this batch row, half of either piece
-  for (int i = tid; i < nslots * D.units * 4; i += LMA_NT) {
-    const int unit = i >> 2, piece = (i >> 1) & 1, half = i & 1;
+  const int any = __syncthreads_or(nan);                             // (and s_h and s_mine are there)
+  if (tid == 0) D.row_nan[p] = any;
+  // 16 bytes at a time, half of a unit's row of either piece: this row of the runs whose 32s hold it
+  const int at = p - g0;
+  for (int i = tid; i < nruns * D.units * 4; i += LMA_NT) {
+    const int unit = i >> 2, piece = (i >> 1) & 1, half = i & 1, q = unit / D.units;
+    if (at < (s_start[q] & ~31) || at >= ((s_start[q + 1] + 31) & ~31)) continue;
     uint32_t o[4] = {0u, 0u, 0u, 0u};
-    if (unit / D.units == s_mine) {
-      const int r0 = (unit % D.units) * LMA_UNIT + half * 8;
+    if (q == s_mine) {
+      const int r0 = (unit - q * D.units) * LMA_UNIT + half * 8;
 #pragma unroll
       for (int c = 0; c < 8; c++) {
         const float v = (r0 + c < D.rank) ? s_h[r0 + c] : 0.0f;
@@ -210,38 +272,79 @@ __global__ void __launch_bounds__(LMA_NT) lm_adapters_kernel(const __grid_consta
         o[c >> 1] |= bits << (16 * (c & 1));
       }
     }
-    uint4* dst = reinterpret_cast<uint4*>(D.h + lma_h_row(D, item_n, g, unit, piece, b - g0) * LMA_UNIT) + half;
+    uint4* dst = reinterpret_cast<uint4*>(D.h + lma_h_row(D, g, unit, piece, at) * LMA_UNIT) + half;
     *dst = make_uint4(o[0], o[1], o[2], o[3]);
   }
 }
 
-// One logit from its row's own operands, in f32.
-__device__ __noinline__ float lma_logit(const LmAdaptArgs& D, int K, int item_n, int b, int v) {
-  const uint4 *x4 = reinterpret_cast<const uint4*>(D.x + b * D.ldx), *w4 = reinterpret_cast<const uint4*>(D.w + v * D.ldw);
+// One logit from its row's own operands, in f32; p: the row's place in the order.
+__device__ __noinline__ float lma_logit(const LmAdaptArgs& D, int p, int v) {
+  const uint4 *x4 = reinterpret_cast<const uint4*>(D.xs + static_cast<int64_t>(p) * D.K), *w4 = reinterpret_cast<const uint4*>(D.w + v * D.ldw);
   float acc = 0.0f;
-  for (int k = 0; k < K / 8; k++) {
-    const uint4 p = __ldg(x4 + k), q = __ldg(w4 + k);
-    const uint32_t ps[4] = {p.x, p.y, p.z, p.w}, qs[4] = {q.x, q.y, q.z, q.w};
+  for (int k = 0; k < D.K / 8; k++) {
+    const uint4 q = x4[k], t = __ldg(w4 + k);
+    const uint32_t qs[4] = {q.x, q.y, q.z, q.w}, ts[4] = {t.x, t.y, t.z, t.w};
 #pragma unroll
-    for (int c = 0; c < 4; c++) { acc = fmaf(bf16_lo(ps[c]), bf16_lo(qs[c]), acc); acc = fmaf(bf16_hi(ps[c]), bf16_hi(qs[c]), acc); }
+    for (int c = 0; c < 4; c++) { acc = fmaf(bf16_lo(qs[c]), bf16_lo(ts[c]), acc); acc = fmaf(bf16_hi(qs[c]), bf16_hi(ts[c]), acc); }
   }
-  const int a = D.row_adapter[b];
-  if (a < 0 || a >= D.n) return acc;
-  const int g = b / item_n;
-  const int32_t* rec = D.groups + static_cast<int64_t>(g) * (LMA_HDR + item_n);
-  int slot = 0;
-  while (slot < rec[0] - 1 && rec[LMA_HDR + slot] != a) slot++;
+  const int a = D.sorted[p];
+  if (a < 0) return acc;
+  const int g = p / D.item_n;
+  const LmaRun* runs = D.runs + static_cast<int64_t>(g) * D.max_runs;
+  int run = 0;
+  while (run < D.nruns[g] - 1 && runs[run].adapter != a) run++;
   const uint16_t* brow = D.b + a * D.b_stride + v * D.b_pitch;
   for (int r = 0; r < D.rank; r++) {
-    const int unit = slot * D.units + r / LMA_UNIT;
     float h = 0.0f;                                                    // (the two parts' sum is exact)
 #pragma unroll
     for (int piece = 0; piece < 2; piece++)
-      h += __uint_as_float(static_cast<uint32_t>(D.h[lma_h_row(D, item_n, g, unit, piece, b - g * item_n) * LMA_UNIT + r % LMA_UNIT]) << 16);
+      h += __uint_as_float(static_cast<uint32_t>(D.h[lma_h_row(D, g, run * D.units + r / LMA_UNIT, piece, p - g * D.item_n) * LMA_UNIT + r % LMA_UNIT]) << 16);
     acc = fmaf(h, __uint_as_float(static_cast<uint32_t>(__ldg(brow + r)) << 16), acc);
   }
   return acc;
 }
+
+// A group's runs in shared memory, one table for each of the threads that walk them: a trip to L2 for every run of every
+// item was much of the time (64 rows with eight adapters: 106 us with, 92 without).
+struct LmaTable { int32_t adapter[LMA_NT]; uint16_t n0[LMA_NT], n1[LMA_NT]; int32_t group, nruns; };
+__device__ __forceinline__ void lma_fetch_runs(LmaTable& t, const LmAdaptArgs& D, int g) {
+  if (t.group == g) return;
+  t.group = g;
+  t.nruns = D.nruns[g];
+  const LmaRun* runs = D.runs + static_cast<int64_t>(g) * D.max_runs;
+#pragma unroll 8
+  for (int i = 0; i < t.nruns; i++) {
+    const int4 r = *reinterpret_cast<const int4*>(runs + i);
+    t.adapter[i] = r.x;
+    t.n0[i] = static_cast<uint16_t>(r.y);
+    t.n1[i] = static_cast<uint16_t>(r.z);
+  }
+}
+// The units of an item, in order: every run that has rows among the item's, and its share of them. The producers and the issuer
+// walk them alike.
+struct LmaUnits {
+  const LmaTable& t;
+  int units, g, i0, i1, run, nruns, ru, n0, n1, adapter;
+  __device__ __forceinline__ LmaUnits(LmaTable& table, const LmAdaptArgs& D, int b0, int n) : t(table) {
+    g = b0 / D.item_n; i0 = b0 - g * D.item_n; i1 = i0 + n;
+    lma_fetch_runs(table, D, g);
+    nruns = t.nruns;
+    units = D.units;
+    run = -1;
+    ru = units - 1;
+  }
+  __device__ __forceinline__ bool next() {
+    if (++ru < units) return run < nruns;
+    ru = 0;
+    while (++run < nruns) {
+      adapter = t.adapter[run];
+      n0 = max(static_cast<int>(t.n0[run]), i0);
+      n1 = min(static_cast<int>(t.n1[run]), i1);
+      if (n0 < n1) return true;
+    }
+    return false;
+  }
+};
 
 // Work items in the order in which pair p takes them: p, p + npairs, ...: first the whole rounds of full
 // items (all batch rows of `full` vocabulary tiles, item_n at a time), then the remaining tiles in items
@@ -345,8 +448,8 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
       : "r"(taddr) : "memory");
 }
 
-// ADAPT: with D's adapters (D is null otherwise). It is then launched as a dependent of the kernel that makes h, with x and w there
-// before, and the products over K go on without waiting for it.
+// ADAPT: with D's adapters (D is null otherwise). It is then launched as a dependent of the kernel that puts the rows in order, with w
+// there before.
 template <bool ADAPT>
 __device__ __forceinline__ void lm_head_run(const LmHeadArgs& A, const LmAdaptArgs* D) {
   extern __shared__ __align__(16) unsigned char lmh_dyn[];
@@ -356,6 +459,9 @@ __device__ __forceinline__ void lm_head_run(const LmHeadArgs& A, const LmAdaptAr
   __shared__ __align__(16) float stash_thr[LMH_EPI][32];
   __shared__ uint2 stash[LMH_EPI][64];
   __shared__ int stash_row[LMH_EPI][64];
+  __shared__ __align__(16) unsigned char lma_space[ADAPT ? (2 + LMA_STAGE) * sizeof(LmaTable) : 16];
+  __shared__ uint32_t lma_given;                                        // stages of units that the producer has found free and announced
+  LmaTable* lma_tables = reinterpret_cast<LmaTable*>(lma_space);     // warp 0's, warp 1's, and of those that ask for units
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t rank = blockIdx.x & 1u;                                // in the pair; 0 leads
   const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
@@ -375,6 +481,10 @@ __device__ __forceinline__ void lm_head_run(const LmHeadArgs& A, const LmAdaptAr
     for (int s = 0; s < nst; s++) { mbar_init(smem_addr(&full_bar[s]), 1); mbar_init(smem_addr(&empty_bar[s]), 1); }
     for (int b = 0; b < 2; b++) { mbar_init(smem_addr(&acc_full[b]), 1); mbar_init(smem_addr(&acc_empty[b]), 2 * LMH_EPI); }
     abort_s = 0;
+    if constexpr (ADAPT) {
+      for (int t = 0; t < 2 + LMA_STAGE; t++) lma_tables[t].group = -1;
+      lma_given = 0;
+    }
     if (A.clear_status && blockIdx.x == 0) *A.status = 0u;              // (a wait runs out seconds later, if ever)
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -395,40 +505,94 @@ __device__ __forceinline__ void lm_head_run(const LmHeadArgs& A, const LmAdaptAr
       asm volatile("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(pol_x));
       if (plan.nb > 1) asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(pol_w));
       uint32_t stage = 0, phase = 0;
+      [[maybe_unused]] uint32_t given = 0;                              // stages of units handed on
       bool ok = true;
       for (int i = pair; i < plan.total && ok; i += npairs) {
         const LmhItem it = plan.at(i);
         const int v0 = ((A.tile0 + it.vt * A.tile_step) * 2 + static_cast<int>(rank)) * A.cta_v;
         const int xb = it.b0 + static_cast<int>(rank) * (it.n >> 1);
+        int asked = 0;
+        if constexpr (ADAPT) {
+          if (i == pair) {                                              // the first stages' weights ahead of the wait for x in its order
+            asked = min(nst, nkc);
+            for (int kc = 0; kc < asked; kc++) {
+              const uint32_t own = smem_addr(&full_bar[kc]), bar = map_rank(own, 0);
+              const int subs = min(LMH_SUB, nk64 - kc * LMH_SUB);
+              if (rank == 0) mbar_expect_tx(own, 2 * subs * (static_cast<uint32_t>(A.cta_v) * LMH_BK * 2 + x_bytes));
+              for (int u = 0; u < subs; u++) tma_load_2d_pair(ring + kc * stage_bytes + u * LMH_W_BYTES, &A.map_w, bar, (kc * LMH_SUB + u) * LMH_BK, v0, pol_w);
+            }
+            pdl_wait();
+          }
+        }
         for (int kc = 0; kc < nkc; kc++) {
-          if (!mbar_wait(smem_addr(&empty_bar[stage]), phase ^ 1u, abort_flag)) { ok = false; break; }
+          if (!ADAPT || kc >= asked) if (!mbar_wait(smem_addr(&empty_bar[stage]), phase ^ 1u, abort_flag)) { ok = false; break; }
           const uint32_t own = smem_addr(&full_bar[stage]), bar = map_rank(own, 0);
           const uint32_t sw = ring + stage * stage_bytes, sx = sw + LMH_SUB * LMH_W_BYTES;
           const int subs = min(LMH_SUB, nk64 - kc * LMH_SUB);
-          if (rank == 0) mbar_expect_tx(own, 2 * subs * (static_cast<uint32_t>(A.cta_v) * LMH_BK * 2 + x_bytes));
-          for (int u = 0; u < subs; u++) tma_load_2d_pair(sw + u * LMH_W_BYTES, &A.map_w, bar, (kc * LMH_SUB + u) * LMH_BK, v0, pol_w);
+          if (!ADAPT || kc >= asked) {
+            if (rank == 0) mbar_expect_tx(own, 2 * subs * (static_cast<uint32_t>(A.cta_v) * LMH_BK * 2 + x_bytes));
+            for (int u = 0; u < subs; u++) tma_load_2d_pair(sw + u * LMH_W_BYTES, &A.map_w, bar, (kc * LMH_SUB + u) * LMH_BK, v0, pol_w);
+          }
           for (int u = 0; u < subs; u++) tma_load_2d_pair(sx + u * x_bytes, &A.map_x, bar, (kc * LMH_SUB + u) * LMH_BK, xb, pol_x);
           if (++stage == static_cast<uint32_t>(nst)) { stage = 0; phase ^= 1u; }
         }
         if constexpr (ADAPT) {
-          pdl_wait();
-          const int g = it.b0 / A.item_n, hrow = it.b0 - g * A.item_n + static_cast<int>(rank) * (it.n >> 1);
-          const int32_t* rec = D->groups + static_cast<int64_t>(g) * (LMA_HDR + A.item_n);
-          const int nu = ok ? rec[0] * D->units : 0;
-          for (int u0 = 0; u0 < nu; u0 += LMA_STAGE) {
+          LmaUnits un(lma_tables[0], *D, it.b0, it.n);
+          bool more = ok && un.next();
+          while (more) {
             if (!mbar_wait(smem_addr(&empty_bar[stage]), phase ^ 1u, abort_flag)) { ok = false; break; }
-            const uint32_t own = smem_addr(&full_bar[stage]), bar = map_rank(own, 0);
-            const uint32_t sw = ring + stage * stage_bytes, sx = sw + LMH_SUB * LMH_W_BYTES, hb = static_cast<uint32_t>(A.box_n) * 32;
-            const int here = min(LMA_STAGE, nu - u0);
-            if (rank == 0) mbar_expect_tx(own, 2 * here * (static_cast<uint32_t>(A.cta_v) * 32 + 2 * hb));
-            for (int u = 0; u < here; u++) {
-              const int slot = (u0 + u) / D->units, ru = (u0 + u) - slot * D->units;
-              tma_load_3d_pair(sw + u * (LMH_CTA_V * 32), &D->map_b, bar, ru * LMA_UNIT, v0, rec[LMA_HDR + slot], pol_w);
-              for (int piece = 0; piece < 2; piece++)
-                tma_load_2d_pair(sx + (2 * u + piece) * hb, &D->map_h, bar, 0, static_cast<int>(lma_h_row(*D, A.item_n, g, u0 + u, piece, hrow)), pol_x);
-            }
+            uint32_t bytes = 0;
+            for (int u = 0; u < LMA_STAGE && more; u++, more = un.next()) bytes += static_cast<uint32_t>(A.cta_v) * 32 + static_cast<uint32_t>(un.n1 - un.n0) * 32;
+            // (the pair's other CTA may have its copies there before this says how many there are: the phase waits for this arrival)
+            if (rank == 0) mbar_expect_tx(smem_addr(&full_bar[stage]), 2 * bytes);
+            given++;
+            asm volatile("st.release.cta.shared.u32 [%0], %1;" :: "r"(smem_addr(&lma_given)), "r"(given) : "memory");
             if (++stage == static_cast<uint32_t>(nst)) { stage = 0; phase ^= 1u; }
           }
+        }
+      }
+    }
+  } else if (ADAPT && warp >= LMH_NT / 32) {
+    // ---- who asks for the units: warp j for the j-th of every stage. (Which stages are free is the producer's word: one of these
+    // could be rounds ahead of a barrier, and its parity would not say so.)
+    if (lane == 0) {
+      const int j = warp - LMH_NT / 32;
+      unsigned long long pol_w, pol_x;
+      asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(pol_w));
+      asm volatile("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(pol_x));
+      if (plan.nb > 1) asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(pol_w));
+      uint32_t stage = 0, seen = 0;                                     // seen: stages of units so far
+      bool ok = true;
+      const uint32_t hb = static_cast<uint32_t>(A.box_n) * 32;
+      pdl_wait();
+      for (int i = pair; i < plan.total && ok; i += npairs) {
+        const LmhItem it = plan.at(i);
+        const int v0 = ((A.tile0 + it.vt * A.tile_step) * 2 + static_cast<int>(rank)) * A.cta_v;
+        stage = (stage + static_cast<uint32_t>(nkc)) % nst;
+        LmaUnits un(lma_tables[2 + j], *D, it.b0, it.n);
+        bool more = un.next();
+        while (more && ok) {
+          const uint32_t sw = ring + stage * stage_bytes, sx = sw + LMH_SUB * LMH_W_BYTES, bar = map_rank(smem_addr(&full_bar[stage]), 0);
+          for (int u = 0; u < LMA_STAGE && more; u++, more = un.next()) {
+            if (u != j) continue;
+            uint32_t have = 0;
+            for (uint32_t polls = 0;; polls++) {
+              asm volatile("ld.acquire.cta.shared.u32 %0, [%1];" : "=r"(have) : "r"(smem_addr(&lma_given)) : "memory");
+              if (have > seen) break;
+              __nanosleep(32);
+              if (polls == LMH_WAIT_LIMIT || *abort_flag) { *abort_flag = 1; ok = false; break; }
+            }
+            if (!ok) break;
+            const int half = (un.n1 - un.n0) >> 1, r0 = un.n0 + static_cast<int>(rank) * half;   // this CTA's batch rows of the unit
+            tma_load_3d_pair(sw + u * (LMH_CTA_V * 32), &D->map_b, bar, un.ru * LMA_UNIT, v0, un.adapter, pol_w);
+            const int hrow = static_cast<int>(lma_h_row(*D, un.g, un.run * D->units + un.ru, 0, r0));
+            for (int q = 0; q < half; q += LMA_BOX) {
+              tma_load_2d_pair(sx + 2 * u * hb + q * 32, &D->map_h, bar, 0, hrow + q, pol_x);
+              tma_load_2d_pair(sx + (2 * u + 1) * hb + q * 32, &D->map_h, bar, 0, hrow + A.item_n + q, pol_x);
+            }
+          }
+          seen++;
+          if (++stage == static_cast<uint32_t>(nst)) stage = 0;
         }
       }
     }
@@ -457,15 +621,17 @@ __device__ __forceinline__ void lm_head_run(const LmHeadArgs& A, const LmAdaptAr
         }
         if constexpr (ADAPT) {
           pdl_wait();
-          const int nu = ok ? D->groups[static_cast<int64_t>(plan.at(i).b0 / A.item_n) * (LMA_HDR + A.item_n)] * D->units : 0;
-          for (int u0 = 0; u0 < nu; u0 += LMA_STAGE) {
+          const LmhItem it = plan.at(i);
+          LmaUnits un(lma_tables[1], *D, it.b0, it.n);
+          bool more = ok && un.next();
+          while (more) {
             if (!mbar_wait(smem_addr(&full_bar[stage]), phase, abort_flag)) { ok = false; break; }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t sw = ring + stage * stage_bytes, sx = sw + LMH_SUB * LMH_W_BYTES, hb = static_cast<uint32_t>(A.box_n) * 32;
-            const int here = min(LMA_STAGE, nu - u0);
-            for (int u = 0; u < here; u++) {
+            for (int u = 0; u < LMA_STAGE && more; u++, more = un.next()) {
               for (int piece = 0; piece < 2; piece++)
-                umma_f16_pair(d_tmem, umma_desc_32b(sw + u * (LMH_CTA_V * 32)), umma_desc_32b(sx + (2 * u + piece) * hb), idesc, 1u);
+                umma_f16_pair(d_tmem + static_cast<uint32_t>(un.n0 - un.i0), umma_desc_32b(sw + u * (LMH_CTA_V * 32)), umma_desc_32b(sx + (2 * u + piece) * hb),
+                              lmh_idesc(un.n1 - un.n0), 1u);
             }
             umma_commit_pair(smem_addr(&empty_bar[stage]));
             if (++stage == static_cast<uint32_t>(nst)) { stage = 0; phase ^= 1u; }
@@ -500,7 +666,7 @@ __device__ __forceinline__ void lm_head_run(const LmHeadArgs& A, const LmAdaptAr
     for (int i = pair; i < plan.total && ok; i += npairs) {
       const LmhItem it = plan.at(i);
       bool adapted = false;
-      if constexpr (ADAPT) adapted = D->groups[static_cast<int64_t>(it.b0 / A.item_n) * (LMA_HDR + A.item_n)] > 0;
+      if constexpr (ADAPT) adapted = D->nruns[it.b0 / A.item_n] > 0;
       if (!mbar_wait(smem_addr(&acc_full[acc]), acc_phase, abort_flag)) { ok = false; break; }
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const int in_tile = static_cast<int>(rank) * A.cta_v + q * 32 + lane;
@@ -522,7 +688,7 @@ __device__ __forceinline__ void lm_head_run(const LmHeadArgs& A, const LmAdaptAr
 #pragma unroll 1
               for (int j = 0; j < nb; j++) {
                 if (!((bad >> j) & 1u) || D->row_nan[b0 + j]) continue;
-                const uint32_t y = __float_as_uint(lma_logit(*D, A.K, A.item_n, b0 + j, v));
+                const uint32_t y = __float_as_uint(lma_logit(*D, b0 + j, v));
 #pragma unroll
                 for (int jj = 0; jj < 32; jj++) r[jj] = (j == jj) ? y : r[jj];
               }
@@ -530,7 +696,14 @@ __device__ __forceinline__ void lm_head_run(const LmHeadArgs& A, const LmAdaptAr
             __syncwarp();
           }
         }
-        if (A.out_logits && live) {
+        if constexpr (ADAPT) {                                         // to the rows' own places
+          const int mine = lane < nb ? D->order[b0 + lane] : 0;
+#pragma unroll
+          for (int j = 0; j < 32; j++) {
+            const int64_t to = __shfl_sync(FULL, mine, j);
+            if (j < nb && live) __stcs(A.out_logits + to * A.ld_out + ocol, __uint_as_float(r[j]));
+          }
+        } else if (A.out_logits && live) {
           float* dst = A.out_logits + static_cast<int64_t>(b0) * A.ld_out + ocol;
           if (nb == 32) {
 #pragma unroll
@@ -607,7 +780,7 @@ __device__ __forceinline__ void lm_head_run(const LmHeadArgs& A, const LmAdaptAr
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LMH_NT, 1) lm_head_kernel(const __grid_constant__ LmHeadArgs A) {
   lm_head_run<false>(A, nullptr);
 }
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LMH_NT, 1) lm_head_adapters_kernel(const __grid_constant__ LmHeadArgs A, const __grid_constant__ LmAdaptArgs D) {
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LMA_RUN_NT, 1) lm_head_adapters_kernel(const __grid_constant__ LmHeadArgs A, const __grid_constant__ LmAdaptArgs D) {
   lm_head_run<true>(A, &D);
 }
 

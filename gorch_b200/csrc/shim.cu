@@ -745,7 +745,7 @@ int launch_lm_head(Ctx* c, gs::LmHeadArgs& a, char** errOut, bool dependent, boo
   a.status = c->host_words;
   a.chained = chained ? 1 : 0;
   a.clear_status = chained && !d ? 0 : 1;
-  if (d) CUDA_TRY(launch(c, gs::lm_head_adapters_kernel, static_cast<unsigned>(2 * npairs), gs::LMH_NT, gs::LMH_DYN_BYTES, dependent, a, *d), errOut);
+  if (d) CUDA_TRY(launch(c, gs::lm_head_adapters_kernel, static_cast<unsigned>(2 * npairs), gs::LMA_RUN_NT, gs::LMA_DYN_BYTES, dependent, a, *d), errOut);
   else CUDA_TRY(launch(c, gs::lm_head_kernel, static_cast<unsigned>(2 * npairs), gs::LMH_NT, gs::LMH_DYN_BYTES, dependent, a), errOut);
   c->counters.kernel_launches += 1;
   return GORCH_CUDA_OK;
@@ -864,7 +864,7 @@ GorchCudaCtxRef gorch_cuda_create_ctx(int device, char** errOut) {
   if ((e = cudaFuncSetAttribute(gs::w1024::wide_rows_kernel<float>, cudaFuncAttributeMaxDynamicSharedMemorySize, gs::w1024::W_DYN_BYTES)) != cudaSuccess) return fail("cudaFuncSetAttribute", e);
   if ((e = cudaFuncSetAttribute(gs::w1024::wide_rows_kernel<uint16_t>, cudaFuncAttributeMaxDynamicSharedMemorySize, gs::w1024::W_DYN_BYTES)) != cudaSuccess) return fail("cudaFuncSetAttribute", e);
   if ((e = cudaFuncSetAttribute(gs::lm_head_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, gs::LMH_DYN_BYTES)) != cudaSuccess) return fail("cudaFuncSetAttribute", e);
-  if ((e = cudaFuncSetAttribute(gs::lm_head_adapters_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, gs::LMH_DYN_BYTES)) != cudaSuccess) return fail("cudaFuncSetAttribute", e);
+  if ((e = cudaFuncSetAttribute(gs::lm_head_adapters_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, gs::LMA_DYN_BYTES)) != cudaSuccess) return fail("cudaFuncSetAttribute", e);
   if ((e = cudaFuncSetAttribute(gs::lmh_finish_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, gs::LMH_F_DYN_BYTES)) != cudaSuccess) return fail("cudaFuncSetAttribute", e);
   if ((e = cudaFuncSetAttribute(gs::row_softmax_kernel<float>, cudaFuncAttributeMaxDynamicSharedMemorySize, gs::RS_DYN_BYTES)) != cudaSuccess) return fail("cudaFuncSetAttribute", e);
   if ((e = cudaFuncSetAttribute(gs::row_softmax_kernel<uint16_t>, cudaFuncAttributeMaxDynamicSharedMemorySize, gs::RS_DYN_BYTES)) != cudaSuccess) return fail("cudaFuncSetAttribute", e);
@@ -1931,17 +1931,24 @@ int gorch_cuda_lm_head_logits_dev(GorchCudaCtxRef ctx, const void* x, int64_t ld
   return launch_lm_head(c, a, errOut, true);
 }
 
-// The workspace of a call with adapters: [group records | NaN marks of the rows | h], for groups of item_n batch rows.
-struct AdapterSpace { int64_t item_n, groups, units, max_units, off_nan, off_h, bytes; };
-static AdapterSpace adapter_space(int64_t B, const GorchAdapters* ad) {
+// The workspace of a call with adapters, for groups of item_n batch rows: [runs per group | runs | order | sorted | NaN marks | x | h].
+struct AdapterSpace { int64_t item_n, groups, units, max_runs, off_runs, off_order, off_sorted, off_nan, off_x, off_h, bytes; };
+static AdapterSpace adapter_space(int64_t B, int64_t K, const GorchAdapters* ad) {
   AdapterSpace s;
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) { const int64_t here = at; at = (at + bytes + 255) & ~255ll; return here; };
   s.item_n = B >= gs::LMH_MAX_N ? gs::LMH_MAX_N : (B + 31) & ~31ll;
   s.groups = (B + s.item_n - 1) / s.item_n;
   s.units = (ad->rank + gs::LMA_UNIT - 1) / gs::LMA_UNIT;
-  s.max_units = (ad->n < s.item_n ? ad->n : s.item_n) * s.units;
-  s.off_nan = (s.groups * (gs::LMA_HDR + s.item_n) * 4 + 255) & ~255ll;
-  s.off_h = (s.off_nan + B * 4 + 255) & ~255ll;
-  s.bytes = s.off_h + s.groups * s.max_units * 2 * s.item_n * gs::LMA_UNIT * 2;
+  s.max_runs = ad->n < s.item_n ? ad->n : s.item_n;
+  take(s.groups * 4);
+  s.off_runs = take(s.groups * s.max_runs * static_cast<int64_t>(sizeof(gs::LmaRun)));
+  s.off_order = take(B * 4);
+  s.off_sorted = take(B * 4);
+  s.off_nan = take(B * 4);
+  s.off_x = take(B * K * 2);
+  s.off_h = take(s.groups * s.max_runs * s.units * 2 * s.item_n * gs::LMA_UNIT * 2);
+  s.bytes = at;
   return s;
 }
 
@@ -1964,13 +1971,16 @@ static int check_adapters(const GorchAdapters* ad, int64_t V, int64_t K, char** 
   return GORCH_CUDA_OK;
 }
 
-int gorch_cuda_lm_head_adapters_workspace(int64_t B, const GorchAdapters* adapters, uint64_t* bytes, char** errOut) {
+int gorch_cuda_lm_head_adapters_workspace(int64_t B, int64_t K, const GorchAdapters* adapters, uint64_t* bytes, char** errOut) {
   if (!bytes) { set_err(errOut, "gorch_cuda: null pointer argument"); return GORCH_CUDA_ERR_BAD_ARG; }
   const int rc = check_adapters(adapters, 0, 0, errOut);
   if (rc) return rc;
-  if (B < 0) { set_err(errOut, "gorch_cuda: bad batch size %lld", (long long)B); return GORCH_CUDA_ERR_BAD_ARG; }
-  if (B > 0x7fffffffll) { set_err(errOut, "gorch_cuda: batch beyond 31 bits"); return GORCH_CUDA_ERR_LIMIT; }
-  *bytes = B == 0 ? 0 : static_cast<uint64_t>(adapter_space(B, adapters).bytes);
+  if (B < 0 || K < gs::LMH_BK || (K % gs::LMH_BK) != 0) {
+    set_err(errOut, "gorch_cuda: LM head needs B >= 0 and K a multiple of %d (got B=%lld K=%lld)", gs::LMH_BK, (long long)B, (long long)K);
+    return GORCH_CUDA_ERR_BAD_ARG;
+  }
+  if (B > 0x7fffffffll || K > 0x7fffffffll) { set_err(errOut, "gorch_cuda: LM head shape beyond 31 bits"); return GORCH_CUDA_ERR_LIMIT; }
+  *bytes = B == 0 ? 0 : static_cast<uint64_t>(adapter_space(B, K, adapters).bytes);
   return GORCH_CUDA_OK;
 }
 
@@ -1988,19 +1998,22 @@ int gorch_cuda_lm_head_adapters_dev(GorchCudaCtxRef ctx, const void* x, int64_t 
     set_err(errOut, "gorch_cuda: row_adapter and the output must be 4-byte aligned, the workspace 256-byte aligned");
     return GORCH_CUDA_ERR_BAD_ARG;
   }
-  const AdapterSpace sp = adapter_space(B, adapters);
+  const AdapterSpace sp = adapter_space(B, K, adapters);
   if (workspace_bytes < static_cast<uint64_t>(sp.bytes)) {
     set_err(errOut, "gorch_cuda: workspace of %llu bytes, %lld needed", (unsigned long long)workspace_bytes, (long long)sp.bytes);
     return GORCH_CUDA_ERR_BAD_ARG;
   }
-  const int64_t h_rows = sp.groups * sp.max_units * 2 * sp.item_n;
+  const int64_t h_rows = sp.groups * sp.max_runs * sp.units * 2 * sp.item_n;
   if (h_rows > 0x7fffffffll) { set_err(errOut, "gorch_cuda: more adapters and batch rows than 31 bits of workspace rows hold"); return GORCH_CUDA_ERR_LIMIT; }
   CUDA_TRY(cudaSetDevice(c->device), errOut);
   if ((rc = load_encode_tiled(errOut))) return rc;
   gs::LmHeadArgs a;
-  if ((rc = lm_head_args(c, a, x, ldx, w, ldw, B, V, K, true, errOut))) return rc;
+  unsigned char* base = static_cast<unsigned char*>(workspace);
+  if ((rc = lm_head_args(c, a, base + sp.off_x, K, w, ldw, B, V, K, true, errOut))) return rc;
   a.tile0 = 0; a.tile_step = 1; a.ntile = static_cast<int32_t>((V + 2 * a.cta_v - 1) / (2 * a.cta_v));
   a.out_logits = out_logits; a.ld_out = ld_out; a.compact = 0;
+  const int stage = gs::LMH_SUB * (gs::LMH_W_BYTES + a.box_n * gs::LMH_BK * 2);
+  if (a.stages > gs::LMA_RING_BYTES / stage) a.stages = gs::LMA_RING_BYTES / stage;
   gs::LmAdaptArgs d;
   memset(&d, 0, sizeof d);
   d.x = static_cast<const uint16_t*>(x); d.w = static_cast<const uint16_t*>(w); d.ldx = ldx; d.ldw = ldw;
@@ -2010,15 +2023,24 @@ int gorch_cuda_lm_head_adapters_dev(GorchCudaCtxRef ctx, const void* x, int64_t 
   d.b_stride = adapters->n > 1 ? adapters->b_stride : V * adapters->b_pitch;
   d.scales = adapters->scales; d.row_adapter = row_adapter;
   d.n = static_cast<int32_t>(adapters->n); d.rank = static_cast<int32_t>(adapters->rank);
-  d.units = static_cast<int32_t>(sp.units); d.max_units = static_cast<int32_t>(sp.max_units);
-  unsigned char* base = static_cast<unsigned char*>(workspace);
-  d.groups = reinterpret_cast<int32_t*>(base);
+  d.units = static_cast<int32_t>(sp.units); d.max_runs = static_cast<int32_t>(sp.max_runs);
+  d.B = a.B; d.K = a.K; d.item_n = a.item_n;
+  d.nruns = reinterpret_cast<int32_t*>(base);
+  d.runs = reinterpret_cast<gs::LmaRun*>(base + sp.off_runs);
+  d.order = reinterpret_cast<int32_t*>(base + sp.off_order);
+  d.sorted = reinterpret_cast<int32_t*>(base + sp.off_sorted);
   d.row_nan = reinterpret_cast<int32_t*>(base + sp.off_nan);
+  d.xs = reinterpret_cast<uint16_t*>(base + sp.off_x);
   d.h = reinterpret_cast<uint16_t*>(base + sp.off_h);
   if ((rc = make_unit_map(&d.map_b, adapters->b, adapters->rank, V, adapters->b_pitch, adapters->n, d.b_stride, a.cta_v, errOut))) return rc;
-  if ((rc = make_unit_map(&d.map_h, d.h, gs::LMA_UNIT, h_rows, gs::LMA_UNIT, 0, 0, a.box_n, errOut))) return rc;
-  // (not a dependent: what it has waited for, the projection behind it reads without waiting)
-  CUDA_TRY(launch(c, gs::lm_adapters_kernel, static_cast<unsigned>(B), gs::LMA_NT, 0, false, d, a.B, a.K, a.item_n), errOut);
+  if ((rc = make_unit_map(&d.map_h, d.h, gs::LMA_UNIT, h_rows, gs::LMA_UNIT, 0, 0, gs::LMA_BOX, errOut))) return rc;
+  // The first kernel is no dependent: the projection reads w, and the second x, without a wait for what came before the call.
+  const bool several = sp.groups > 1;
+  if (several) {
+    CUDA_TRY(launch(c, gs::lm_adapters_order_kernel, static_cast<unsigned>((B + gs::LMA_NT - 1) / gs::LMA_NT), gs::LMA_NT, 0, false, d), errOut);
+    c->counters.kernel_launches += 1;
+  }
+  CUDA_TRY(launch(c, gs::lm_adapters_kernel, static_cast<unsigned>(B), gs::LMA_NT, 0, several, d, several ? 1 : 0), errOut);
   c->counters.kernel_launches += 1;
   return launch_lm_head(c, a, errOut, true, true, &d);
 }

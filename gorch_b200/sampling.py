@@ -410,10 +410,10 @@ class CudaSampler:
         rc = self._lib.gorch_cuda_lm_head_logits_dev(self._ctx, x_ptr, ldx, w_ptr, ldw, B, V, K, out_ptr, ld_out, C.byref(err))
         _check(self._lib, rc, err)
 
-    def lm_head_adapters_workspace(self, B: int, adapters) -> int:
-        """gorch_cuda_lm_head_adapters_workspace: bytes of device memory that lm_head_adapters_ptrs needs for B rows."""
+    def lm_head_adapters_workspace(self, B: int, K: int, adapters) -> int:
+        """gorch_cuda_lm_head_adapters_workspace: bytes of device memory that lm_head_adapters_ptrs needs for B rows of K."""
         n, err = C.c_uint64(0), C.c_void_p()
-        rc = self._lib.gorch_cuda_lm_head_adapters_workspace(B, C.byref(adapters) if adapters is not None else None, C.byref(n), C.byref(err))
+        rc = self._lib.gorch_cuda_lm_head_adapters_workspace(B, K, C.byref(adapters) if adapters is not None else None, C.byref(n), C.byref(err))
         _check(self._lib, rc, err)
         return int(n.value)
 

@@ -461,7 +461,7 @@ typedef struct {
   const float* scales;  /* [n], or NULL: 1 */
   int64_t n, rank;
 } GorchAdapters;
-int gorch_cuda_lm_head_adapters_workspace(int64_t B, const GorchAdapters* adapters, uint64_t* bytes, char** errOut);
+int gorch_cuda_lm_head_adapters_workspace(int64_t B, int64_t K, const GorchAdapters* adapters, uint64_t* bytes, char** errOut);
 int gorch_cuda_lm_head_adapters_dev(GorchCudaCtxRef ctx, const void* x, int64_t ldx, const void* w, int64_t ldw,
                                     int64_t B, int64_t V, int64_t K, const GorchAdapters* adapters,
                                     const int32_t* row_adapter, void* workspace, uint64_t workspace_bytes,

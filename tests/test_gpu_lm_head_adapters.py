@@ -66,7 +66,7 @@ class _Case:
         t.cuda.synchronize()
 
     def space(self, s):
-        ws = self.torch.empty(s.lm_head_adapters_workspace(self.B, self.rec), dtype=self.torch.uint8, device="cuda")
+        ws = self.torch.empty(s.lm_head_adapters_workspace(self.B, self.K, self.rec), dtype=self.torch.uint8, device="cuda")
         return ws.fill_(0xff)                                   # NaN patterns: what is not written must not matter
 
     def call(self, s, ws, out, ld=None):
@@ -262,10 +262,10 @@ def test_refusals(_sampler_session):
                dict(rec=rec(scales=c.rec.scales + 2))):
         with pytest.raises(GorchCudaError):
             call(**kw)
-    for bad in (dict(B=-1), dict(rec=None), dict(rec=rec(n=-1)), dict(rec=rec(rank=300))):
+    for bad in (dict(B=-1), dict(K=65), dict(rec=None), dict(rec=rec(n=-1)), dict(rec=rec(rank=300))):
         with pytest.raises(GorchCudaError):
-            s.lm_head_adapters_workspace(bad.get("B", 4), bad.get("rec", c.rec))
+            s.lm_head_adapters_workspace(bad.get("B", 4), bad.get("K", 64), bad.get("rec", c.rec))
     call(B=0)
-    assert s.lm_head_adapters_workspace(0, c.rec) == 0
+    assert s.lm_head_adapters_workspace(0, 64, c.rec) == 0
     s.sync()
     assert torch.all(out == 7.0)
