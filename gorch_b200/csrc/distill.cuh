@@ -294,8 +294,16 @@ __global__ void __launch_bounds__(DB_NT, 4) distill_bwd_kernel(const __grid_cons
         for (int c = 0; c < VEC; c++) y[c] = 0.0f;
       }
       if (A.accumulate) {
+        if (vec_ok && i0 >= 0 && i0 + VEC <= A.V) {
 #pragma unroll
-        for (int c = 0; c < VEC; c++) if (i0 + c >= 0 && i0 + c < A.V) y[c] += drow[i0 + c];
+          for (int c = 0; c < VEC; c += 4) {
+            const float4 o = *reinterpret_cast<const float4*>(drow + i0 + c);
+            y[c] += o.x; y[c + 1] += o.y; y[c + 2] += o.z; y[c + 3] += o.w;
+          }
+        } else {
+#pragma unroll
+          for (int c = 0; c < VEC; c++) if (i0 + c >= 0 && i0 + c < A.V) y[c] += drow[i0 + c];
+        }
       }
       const uint32_t bits = any ? (s_bits[e0 >> 5] >> (e0 & 31)) & ((1u << VEC) - 1u) : 0u;
       if (bits == 0u) {

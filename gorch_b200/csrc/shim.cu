@@ -1597,7 +1597,9 @@ static int launch_adjust(Ctx* c, const void* logits, int dtype, int64_t B, int64
   if (in_place && !touch && !a.mask) return GORCH_CUDA_OK;
   size_t dyn = 0;
   if (touch) {
-    if (adjust_split(c, a, dtype, B, in_place)) {
+    const bool stream = adjust_split(c, a, dtype, B, in_place);
+    if (B * a.nchunk > 0x7fffffffll) { set_err(errOut, "gorch_cuda: batch beyond the limit of a launch"); return GORCH_CUDA_ERR_LIMIT; }
+    if (stream) {
       const int64_t total = B * a.nchunk;
       const int bytes = gs::al_stream_bytes(a.chunk * (f32 ? 4 : 8), f32 ? 4 : 2, in_place);
       int per = (227 << 10) / (bytes + gs::AL_STREAM_STATIC + 1024);   // CTAs that an SM holds

@@ -397,6 +397,72 @@ def test_a_grammar_that_allows_nothing_ends_its_row(_sampler_session):
         ended.release()
 
 
+def test_generation_with_long_prompts(_sampler_session, oracle):
+    """Token buffers beyond what the kernel for short histories holds, and one beyond 2^15 tokens: the rows' own tokens are the history."""
+    import torch
+    s = _sampler_session
+    rng = np.random.default_rng(77)
+    V, max_new = 9000, 3
+    for longest in (6000, 40000):
+        prompts = [(rng.random(n) ** 3 * V).astype(int).tolist() for n in (longest, 5, 4097, 1)]
+        B = len(prompts)
+        steps = [_logits(rng, B, V, False) for _ in range(max_new)]
+        cfgs = np.zeros(B, dtype=CFG_DTYPE)                     # greedy: the ids follow from the adjusted logits alone
+        pen = np.tile(np.float32([1.3, 0.4, 0.2]), (B, 1))
+        with LogitRules(s, B, penalties=pen) as r:
+            torch.cuda.synchronize()
+            s.set_stream(torch.cuda.current_stream().cuda_stream)
+            try:
+                got = generate_on_device(_Model(torch, steps, DTYPE_F32), prompts, cfgs, np.zeros((max_new, B)), s, max_new, 1 << 20, rules=r)
+            finally:
+                s.set_stream(None)
+        held = [list(p) for p in prompts]
+        for i in range(max_new):
+            y, _ = rules_plain.adjust(steps[i], pen, held, [len(p) for p in prompts], dtype=np.float32)
+            for b in range(B):
+                held[b].append(int(y[b].argmax()))
+        assert got["tokens"] == held
+
+
+def test_rules_of_another_batch_size_are_refused(_sampler_session):
+    s = _sampler_session
+    st = DeviceGenerateState(s, [[1], [2]], 3, 100, (), LOOP_CACHED)
+    try:
+        with LogitRules(s, 1, masks=np.ones((1, 64), bool)) as r:
+            with pytest.raises(ValueError):
+                st.step(16, DTYPE_F32, 64, 64, 16, 16, r)
+            with pytest.raises(ValueError):
+                adjust_logits(s, np.zeros((2, 64), np.float32), r)
+    finally:
+        st.release()
+
+
+@pytest.mark.parametrize("T,stride", [(4096, 4096), (4097, 4097), (4500, 40000), (32767, 32767), (32768, 32768)])
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_histories_around_the_kernels_limits(_sampler_session, T, stride, bf16, in_place):
+    """As many tokens as the registers hold and one more, as 16-bit counts hold and one more; all rules; tokens crowded into a few
+    columns, one of them in every place."""
+    rng = np.random.default_rng(T)
+    B, V = 3, 20000
+    x = _logits(rng, B, V, bf16)
+    rules = _rules(rng, B, V, 50, 400, 2)
+    rules["history"] = [(rng.random(T) ** 6 * V).astype(int).tolist(), [V - 1] * T, list(range(100))]
+    rules["prompt_lengths"] = [T // 3, 1, 200]
+    rules["penalties"] = np.float32([[1.2, 0.3, 0.01], [0.9, 0.0, 0.001], [1.1, -0.2, 0.5]])
+    s = _sampler_session
+    with LogitRules(s, B, **rules) as r:
+        if stride > T:                                          # room for more tokens than there are
+            import torch
+            wide = torch.full((B, stride), 3, dtype=torch.int32)
+            for b, h in enumerate(rules["history"]):
+                wide[b, : len(h)] = torch.tensor(h, dtype=torch.int32)
+            wide = wide.cuda()
+            torch.cuda.synchronize()
+            r.record.history, r.record.history_stride = wide.data_ptr(), stride
+        _check(adjust_logits(s, x, r, in_place), x, **rules)
+
+
 def test_refused_steps_leave_the_logits_alone(_sampler_session):
     import torch
     s = _sampler_session
