@@ -1613,7 +1613,7 @@ static int launch_adjust(Ctx* c, const void* logits, int dtype, int64_t B, int64
     }
     dyn = static_cast<size_t>(gs::al_dyn_bytes(a.chunk * (f32 ? 4 : 8), a.wide != 0, f32 ? 4 : 2, in_place));
   } else {
-    a.chunk = gs::AL_NT * gs::AL_U;
+    a.chunk = in_place ? gs::AL_MASK_CHUNK : gs::AL_NT * gs::AL_U;
     a.nchunk = static_cast<int32_t>((row_vectors(V, dtype) + a.chunk - 1) / a.chunk);
   }
   if (B * a.nchunk > 0x7fffffffll) { set_err(errOut, "gorch_cuda: batch beyond the limit of a launch"); return GORCH_CUDA_ERR_LIMIT; }
