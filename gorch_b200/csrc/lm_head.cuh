@@ -542,9 +542,9 @@ __device__ __forceinline__ void lm_head_run(const LmHeadArgs& A, const LmAdaptAr
           LmaUnits un(lma_tables[0], *D, it.b0, it.n);
           bool more = ok && un.next();
           while (more) {
-            if (!mbar_wait(smem_addr(&empty_bar[stage]), phase ^ 1u, abort_flag)) { ok = false; break; }
             uint32_t bytes = 0;
             for (int u = 0; u < LMA_STAGE && more; u++, more = un.next()) bytes += static_cast<uint32_t>(A.cta_v) * 32 + static_cast<uint32_t>(un.n1 - un.n0) * 32;
+            if (!mbar_wait(smem_addr(&empty_bar[stage]), phase ^ 1u, abort_flag)) { ok = false; break; }
             // (the pair's other CTA may have its copies there before this says how many there are: the phase waits for this arrival)
             if (rank == 0) mbar_expect_tx(smem_addr(&full_bar[stage]), 2 * bytes);
             given++;
@@ -577,17 +577,17 @@ __device__ __forceinline__ void lm_head_run(const LmHeadArgs& A, const LmAdaptAr
           const uint32_t sw = ring + stage * stage_bytes, sx = sw + LMH_SUB * LMH_W_BYTES, bar = map_rank(smem_addr(&full_bar[stage]), 0);
           for (int u = 0; u < LMA_STAGE && more; u++, more = un.next()) {
             if (u != j) continue;
-            uint32_t have = 0;
-            for (uint32_t polls = 0;; polls++) {
+            const int half = (un.n1 - un.n0) >> 1, r0 = un.n0 + static_cast<int>(rank) * half;   // this CTA's batch rows of the unit
+            const int hrow = static_cast<int>(lma_h_row(*D, un.g, un.run * D->units + un.ru, 0, r0));
+            for (uint32_t have = 0, polls = 0; have <= seen; polls++) {
               asm volatile("ld.acquire.cta.shared.u32 %0, [%1];" : "=r"(have) : "r"(smem_addr(&lma_given)) : "memory");
-              if (have > seen) break;
-              __nanosleep(32);
-              if (polls == LMH_WAIT_LIMIT || *abort_flag) { *abort_flag = 1; ok = false; break; }
+              if ((polls & 63u) == 63u) {                               // (a stage comes within a tile's time; after a thousand looks, with pauses)
+                if (polls > 1024u) __nanosleep(200);
+                if (have <= seen && (polls == LMH_WAIT_LIMIT + 63u || *abort_flag)) { *abort_flag = 1; ok = false; break; }
+              }
             }
             if (!ok) break;
-            const int half = (un.n1 - un.n0) >> 1, r0 = un.n0 + static_cast<int>(rank) * half;   // this CTA's batch rows of the unit
             tma_load_3d_pair(sw + u * (LMH_CTA_V * 32), &D->map_b, bar, un.ru * LMA_UNIT, v0, un.adapter, pol_w);
-            const int hrow = static_cast<int>(lma_h_row(*D, un.g, un.run * D->units + un.ru, 0, r0));
             for (int q = 0; q < half; q += LMA_BOX) {
               tma_load_2d_pair(sx + 2 * u * hb + q * 32, &D->map_h, bar, 0, hrow + q, pol_x);
               tma_load_2d_pair(sx + (2 * u + 1) * hb + q * 32, &D->map_h, bar, 0, hrow + A.item_n + q, pol_x);
