@@ -99,10 +99,10 @@ struct LmHeadArgs {
 // on the x side, over the multiple of 32 batch rows that holds the run, with zeros in the rows around it. LMA_STAGE units share a
 // stage of the ring (32-byte rows, 32-byte swizzle; what a rank leaves of a unit is filled with zeros by the copy). Four warps of
 // their own ask for a stage's units, one each, once the producer has found the stage free and announced its bytes (256 rows with 32
-// adapters of rank 32 over 1,024 x 151,936: 247 us so, 355 with one thread asking for all, 401 with cp.async in place of TMA;
-// the projection alone 96). What bounds it: W and the b's are 121 us at the copy rate; a stage's way round the ring, with three
-// stages of 64 KB for 256 rows, is 60 us of the rest, its MMAs 34, its loads 32. 64 rows with eight adapters of rank 16: 91 us (72
-// alone); one row: 71 (65).
+// adapters of rank 32 over 1,024 x 151,936: 225 us so, 355 with one thread asking for all, 401 with cp.async in place of TMA;
+// the projection alone 95). What bounds it: W and the b's are 121 us at the copy rate; a stage's way round the ring, with three
+// stages of 64 KB for 256 rows, is about 50 us of the rest, the MMAs 34, the loads 32 (six or eight units to a stage did not make it
+// faster: 276, 237). 64 rows with eight adapters of rank 16: 90 us (70 alone); one row: 70 (64).
 // So an adapter's b passes once per group, its products cost what its rows cost, rounded up to 32 (with every unit over all
 // rows of the item, 256 x 1,024 x 151,936 with 32 adapters of rank 32 took 290 us), and the epilogue's results are complete.
 // h goes in as two bf16, the rounded value and what the rounding left, each multiplied with the same tile of b: one bf16 would put
