@@ -5,8 +5,9 @@ The package holds only that path and its nearest neighbours: csrc/ (kernels + th
 C ABI of libgorchcuda.so), the ctypes binding, a host-side mirror of the
 reference's sampling interface (sampling.py), the generate loops with their control
 on the device (generate.py), the tensor-level TopK / Multinomial and the row
-softmax / cross-entropy ops (sampling.py, row_ops.py), row and vocab sharding
-(distributed.py), and the seeded synthetic workloads used for measurement.
+softmax / cross-entropy / distillation ops (sampling.py, row_ops.py), the rules of a
+request on its logits (rules.py), row and vocab sharding (distributed.py), and the
+seeded synthetic workloads used for measurement.
 """
 from .config import (CFG_DTYPE, FLAG_BAD_CFG, FLAG_BOUNDARY, FLAG_FALLBACK, FLAG_GENERAL_PATH,
                      FLAG_INTERNAL, FLAG_NONFINITE, FLAG_TIE_CUT, FLAG_TOPP_EDGE,

@@ -9,13 +9,12 @@
 // in f32, each operation rounded once, and one rounding to bf16 at the end for bf16 logits. A logit that no rule
 // touches keeps its bits.
 //
-// Without penalties and biases, adjust_rows_kernel: a stream over every column (out of place; in place it writes what the mask
-// takes away and reads no logit).
+// Without penalties and biases, adjust_rows_kernel: a stream over every column (in place it writes what the mask takes away, and
+// reads the vectors of which the mask keeps some).
 // With them, a CTA takes ranges of a row's columns and counts the tokens that fall into a range in shared memory, a word of 16 or 32
 // bits per column (integer atomics: the order does not matter). Meanwhile the range's logits are on their way to shared
 // memory; the touched ones are changed there, and the range leaves for the output with the mask applied on the way. In place only
-// the touched logits are read, and written where they lie; masked ones are written one by one where the mask takes some of a
-// vector, kept ones never, so that the two do not meet. Two kernels: adjust_stream_kernel for short histories,
+// the touched logits are read, and written where they lie; behind a barrier the mask goes over the range. Two kernels: adjust_stream_kernel for short histories,
 // adjust_touched_kernel, whose CTAs each walk the row's whole history, for long ones.
 // Bound: memory out of place, one read and one write of the row (512 x 151,936 with 1,000 tokens each: bf16 61 us, 5.1 TB/s; f32 106 us, 5.9
 // TB/s; the copy alone 47 and 92); in place, where little is moved, the latency of three trips to L2 one after the other
@@ -37,6 +36,7 @@ constexpr int AL_T_NT = 512;                  // adjust_touched_kernel
 constexpr int AL_T_NW = AL_T_NT / 32;
 constexpr int AL_T_BATCH = 8;                 // its loads of tokens
 constexpr int AL_MASK_CHUNK = 8 * AL_NT;      // adjust_rows_kernel in place: vectors of a CTA
+constexpr int AL_REG_TOKENS = 16 * AL_NT;     // of a row that adjust_stream_kernel takes
 constexpr int AL_U = 4;                       // adjust_rows_kernel: 16-byte vectors per thread
 constexpr int AL_BATCH = 4;                   // touched columns that a lane works on together
 constexpr int AL_LIST = 32 * AL_BATCH + 64;   // touched columns that a warp collects before it works on them
@@ -66,6 +66,7 @@ struct AdjustArgs {
   const int32_t* mask_rows;       // [B] or null: row b has mask b
   const int32_t* row_done;        // [B] or null: rows that are not 0 here are left alone
   int32_t wide;                   // counts of 32 bits: histories of 2^15 tokens and more
+  int32_t shared_out;             // both kernels run: rows of more than AL_REG_TOKENS tokens are adjust_touched_kernel's, the others the other's
 };
 
 __device__ __forceinline__ const uint32_t* al_mask_row(const AdjustArgs& A, int64_t row) {
@@ -244,6 +245,7 @@ __global__ void __launch_bounds__(AL_T_NT) adjust_touched_kernel(const __grid_co
   pdl_launch();
   pdl_wait();                                                        // whatever fills the inputs, or still reads the output
   if (A.row_done != nullptr && A.row_done[row] != 0) return;
+  if (A.shared_out && min(static_cast<int64_t>(A.lengths[row]), A.history_stride) <= AL_REG_TOKENS) return;
   const T* xrow = static_cast<const T*>(A.x) + row * A.row_stride;
   T* orow = static_cast<T*>(A.out) + row * A.out_stride;
   RowView<T> rv;
@@ -425,7 +427,6 @@ __global__ void __launch_bounds__(AL_T_NT) adjust_touched_kernel(const __grid_co
 // counts at zero for the next range. The next ranges' logits are on their way meanwhile.
 // (With a pass over all the row's tokens for every range, 512 x 151,936 bf16 with 1,000 tokens each took 74 us: 630 instructions a
 // warp and range, most of them with a lane or two at work.)
-constexpr int AL_REG_TOKENS = 16 * AL_NT;
 constexpr int AL_STREAM_PER_SM = 4;           // CTAs of 64 registers a thread
 constexpr int AL_BINS = 64;                   // ranges of a row that are sorted for at a time
 constexpr int AL_BUFS = 2;                    // ranges in shared memory: the one worked on, and one on its way
@@ -508,6 +509,7 @@ __global__ void __launch_bounds__(AL_NT, 4) adjust_stream_kernel(const __grid_co
         len = static_cast<int>(min(static_cast<int64_t>(max(A.lengths[row], 0)), A.history_stride));
         if (A.n_new != nullptr) prompt = len - A.n_new[row];
         else if (A.prompt_lengths != nullptr) prompt = A.prompt_lengths[row];
+        if (A.shared_out && len > AL_REG_TOKENS) { live = false; len = off0 = off1 = 0; }
         any = len > 0 && (rep != 1.0f || pres != 0.0f || freq != 0.0f);   // (a row without penalties does not read its history)
       }
       const int n_own = off1 - off0 <= AL_NT ? off1 - off0 : 0;

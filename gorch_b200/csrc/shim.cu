@@ -1560,24 +1560,23 @@ static int check_adjust(const GorchLogitAdjust* adj, int64_t B, int64_t V, bool 
   return GORCH_CUDA_OK;
 }
 
-// The columns of a row that a CTA takes at a time, and which kernel: histories of up to AL_REG_TOKENS tokens (the room for them, which
-// is what the host knows) go to adjust_stream_kernel. us, adjust_touched_kernel | that, in place and out of place, bf16 rows of
-// 151,936: 64 with 2,048 tokens each: 20 | 12, 20 | 16; 512 with 1,000: 100 | 22, 113 | 61. Longer ones do not fit its registers.
-// Ranges of 16 KB where logits are staged (512 x 151,936 bf16 us, 8 | 16 | 24 KB: 75 | 61 | 82, with the CTAs per SM that fit), of 16,384 columns
-// otherwise; fewer where the batch is too small to give every SM two.
-static bool adjust_split(const Ctx* c, gs::AdjustArgs& a, int dtype, int64_t B, bool in_place) {
+// Rows with penalties or biases: histories of up to AL_REG_TOKENS tokens go to adjust_stream_kernel, longer ones do not fit its
+// registers and go to adjust_touched_kernel. The host knows the room for tokens, not the rows' lengths: where there is room for more, both
+// run on large batches, each taking its rows; on small ones the latter alone. us in place and out of place, bf16 rows of 151,936, stream |
+// touched | both: 64 with 2,048 tokens each 12, 16 | 20, 22 | 16, 19; 512 with 1,000: 20, 59 | 110, 131 | 32, 71.
+constexpr int64_t kAdjustBothRows = 64;
+// The columns of a row that a CTA takes at a time: 16 KB of logits where they are staged by adjust_stream_kernel (512 x 151,936 bf16 us, 8 |
+// 16 | 24 KB: 75 | 61 | 82, with the CTAs per SM that fit), 16,384 otherwise; fewer where the batch is too small to give every SM two.
+static void adjust_columns(const Ctx* c, gs::AdjustArgs& a, int dtype, int64_t B, bool staged) {
   const int64_t nvec = row_vectors(a.V, dtype), vec = dtype == GORCH_CUDA_F32 ? 4 : 8;
-  const bool stream = !a.penalties || a.history_stride <= gs::AL_REG_TOKENS;
-  int64_t chunk = stream && !in_place ? gs::AL_STAGE_BYTES / 16 : gs::AL_MAX_COLS / vec;
+  int64_t chunk = staged ? gs::AL_STAGE_BYTES / 16 : gs::AL_MAX_COLS / vec;
   const int64_t spread = (B * nvec / (2 * c->sm_count) + 7) & ~7ll;
   if (chunk > spread) chunk = spread > gs::AL_NT ? spread : gs::AL_NT;
-  a.wide = a.history_stride >= (1 << 15) ? 1 : 0;
   a.chunk = static_cast<int32_t>(chunk);
   a.nchunk = static_cast<int32_t>((nvec + chunk - 1) / chunk);
-  return stream;
 }
 
-// One launch of adjust_rows_kernel or adjust_touched_kernel. gc: the rows' tokens and the rows to pass over come from there.
+// The launches of a call. gc: the rows' tokens and the rows to pass over come from there.
 static int launch_adjust(Ctx* c, const void* logits, int dtype, int64_t B, int64_t V, int64_t row_stride, const GorchLogitAdjust* adj,
                          void* out, int64_t out_stride, const GorchGenControl* gc, char** errOut) {
   gs::AdjustArgs a{};
@@ -1595,36 +1594,39 @@ static int launch_adjust(Ctx* c, const void* logits, int dtype, int64_t B, int64
   if (gc) a.row_done = gc->done;
   const bool in_place = out == logits, touch = a.penalties || a.bias_offsets, f32 = dtype == GORCH_CUDA_F32;
   if (in_place && !touch && !a.mask) return GORCH_CUDA_OK;
-  size_t dyn = 0;
-  if (touch) {
-    const bool stream = adjust_split(c, a, dtype, B, in_place);
-    if (B * a.nchunk > 0x7fffffffll) { set_err(errOut, "gorch_cuda: batch beyond the limit of a launch"); return GORCH_CUDA_ERR_LIMIT; }
-    if (stream) {
-      const int64_t total = B * a.nchunk;
-      const int bytes = gs::al_stream_bytes(a.chunk * (f32 ? 4 : 8), f32 ? 4 : 2, in_place);
-      int per = (227 << 10) / (bytes + gs::AL_STREAM_STATIC + 1024);   // CTAs that an SM holds
-      if (per > gs::AL_STREAM_PER_SM) per = gs::AL_STREAM_PER_SM;
-      const unsigned grid = static_cast<unsigned>(total < per * c->sm_count ? total : per * c->sm_count);
-      auto* k = f32 ? (in_place ? gs::adjust_stream_kernel<float, true> : gs::adjust_stream_kernel<float, false>)
-                    : (in_place ? gs::adjust_stream_kernel<uint16_t, true> : gs::adjust_stream_kernel<uint16_t, false>);
-      CUDA_TRY(launch(c, k, grid, gs::AL_NT, static_cast<size_t>(bytes), true, a, total), errOut);
-      c->counters.kernel_launches += 1;
-      return GORCH_CUDA_OK;
-    }
-    dyn = static_cast<size_t>(gs::al_dyn_bytes(a.chunk * (f32 ? 4 : 8), a.wide != 0, f32 ? 4 : 2, in_place));
-  } else {
+  if (B > 0x7fffffffll / (row_vectors(V, dtype) / gs::AL_NT + 1)) { set_err(errOut, "gorch_cuda: batch beyond the limit of a launch"); return GORCH_CUDA_ERR_LIMIT; }
+  if (!touch) {
     a.chunk = in_place ? gs::AL_MASK_CHUNK : gs::AL_NT * gs::AL_U;
     a.nchunk = static_cast<int32_t>((row_vectors(V, dtype) + a.chunk - 1) / a.chunk);
+    auto* k = f32 ? (in_place ? gs::adjust_rows_kernel<float, true> : gs::adjust_rows_kernel<float, false>)
+                  : (in_place ? gs::adjust_rows_kernel<uint16_t, true> : gs::adjust_rows_kernel<uint16_t, false>);
+    CUDA_TRY(launch(c, k, static_cast<unsigned>(B * a.nchunk), gs::AL_NT, 0, true, a), errOut);
+    c->counters.kernel_launches += 1;
+    return GORCH_CUDA_OK;
   }
-  if (B * a.nchunk > 0x7fffffffll) { set_err(errOut, "gorch_cuda: batch beyond the limit of a launch"); return GORCH_CUDA_ERR_LIMIT; }
-  auto pick = [&](auto type) {
-    typedef decltype(type) E;
-    auto* k = touch ? (in_place ? gs::adjust_touched_kernel<E, true> : gs::adjust_touched_kernel<E, false>)
-                    : (in_place ? gs::adjust_rows_kernel<E, true> : gs::adjust_rows_kernel<E, false>);
-    return launch(c, k, static_cast<unsigned>(B * a.nchunk), touch ? gs::AL_T_NT : gs::AL_NT, dyn, true, a);
-  };
-  CUDA_TRY(f32 ? pick(float()) : pick(uint16_t()), errOut);
-  c->counters.kernel_launches += 1;
+  const bool room = a.penalties && a.history_stride > gs::AL_REG_TOKENS;
+  a.shared_out = room && B >= kAdjustBothRows ? 1 : 0;
+  if (!room || a.shared_out) {
+    adjust_columns(c, a, dtype, B, !in_place);
+    const int64_t total = B * a.nchunk;
+    const int bytes = gs::al_stream_bytes(a.chunk * (f32 ? 4 : 8), f32 ? 4 : 2, in_place);
+    int per = (227 << 10) / (bytes + gs::AL_STREAM_STATIC + 1024);     // CTAs that an SM holds
+    if (per > gs::AL_STREAM_PER_SM) per = gs::AL_STREAM_PER_SM;
+    const unsigned grid = static_cast<unsigned>(total < per * c->sm_count ? total : per * c->sm_count);
+    auto* k = f32 ? (in_place ? gs::adjust_stream_kernel<float, true> : gs::adjust_stream_kernel<float, false>)
+                  : (in_place ? gs::adjust_stream_kernel<uint16_t, true> : gs::adjust_stream_kernel<uint16_t, false>);
+    CUDA_TRY(launch(c, k, grid, gs::AL_NT, static_cast<size_t>(bytes), true, a, total), errOut);
+    c->counters.kernel_launches += 1;
+  }
+  if (room) {
+    adjust_columns(c, a, dtype, B, false);
+    a.wide = a.history_stride >= (1 << 15) ? 1 : 0;
+    const size_t dyn = static_cast<size_t>(gs::al_dyn_bytes(a.chunk * (f32 ? 4 : 8), a.wide != 0, f32 ? 4 : 2, in_place));
+    auto* k = f32 ? (in_place ? gs::adjust_touched_kernel<float, true> : gs::adjust_touched_kernel<float, false>)
+                  : (in_place ? gs::adjust_touched_kernel<uint16_t, true> : gs::adjust_touched_kernel<uint16_t, false>);
+    CUDA_TRY(launch(c, k, static_cast<unsigned>(B * a.nchunk), gs::AL_T_NT, dyn, true, a), errOut);
+    c->counters.kernel_launches += 1;
+  }
   return GORCH_CUDA_OK;
 }
 

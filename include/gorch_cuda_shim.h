@@ -367,7 +367,7 @@ typedef struct {
   const int32_t* mask_rows;      /* [B] the row's mask, outside [0, n_masks): none; or NULL: row b has mask b */
 } GorchLogitAdjust;
 /* out [B,out_stride] has the logits' type; it may be `logits` itself with the same stride (in place:
- * then only what changes is read and written), and must not overlap them otherwise. Device pointers,
+ * then only what changes, and 16-byte vectors that a mask cuts, is read and written), and must not overlap them otherwise. Device pointers,
  * asynchronous on the context's stream, no memory of the context's is used. */
 int gorch_cuda_adjust_logits_dev(GorchCudaCtxRef ctx, const void* logits, int dtype, int64_t B,
                                  int64_t V, int64_t row_stride, const GorchLogitAdjust* adjust,

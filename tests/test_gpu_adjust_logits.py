@@ -463,6 +463,21 @@ def test_histories_around_the_kernels_limits(_sampler_session, T, stride, bf16, 
         _check(adjust_logits(s, x, r, in_place), x, **rules)
 
 
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_short_and_long_histories_in_one_large_batch(_sampler_session, bf16, in_place):
+    """Room for more tokens than the kernel for short histories holds, in a batch that both kernels share: every row once."""
+    rng = np.random.default_rng(4)
+    B, V = 70, 5001
+    x = _logits(rng, B, V, bf16)
+    rules = _rules(rng, B, V, 300, 40, 3)
+    for b, n in ((3, 4096), (4, 4097), (5, 6000), (40, 5000), (69, 4500)):
+        rules["history"][b] = (rng.random(n) ** 3 * V).astype(int).tolist()
+        rules["prompt_lengths"][b] = n // 2
+    rules["penalties"][5] = (1.0, 0.0, 0.0)                     # long, and without a penalty
+    _check(_run(_sampler_session, x, in_place, **rules), x, **rules)
+
+
 def test_refused_steps_leave_the_logits_alone(_sampler_session):
     import torch
     s = _sampler_session
