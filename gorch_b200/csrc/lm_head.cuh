@@ -288,6 +288,7 @@ __device__ __noinline__ float lma_logit(const LmAdaptArgs& D, int p, int v) {
     const uint32_t qs[4] = {q.x, q.y, q.z, q.w}, ts[4] = {t.x, t.y, t.z, t.w};
 #pragma unroll
     for (int c = 0; c < 4; c++) { acc = fmaf(bf16_lo(qs[c]), bf16_lo(ts[c]), acc); acc = fmaf(bf16_hi(qs[c]), bf16_hi(ts[c]), acc); }
+    if (acc != acc) return acc;                                        // (a NaN of the projection's own)
   }
   const int a = D.sorted[p];
   if (a < 0) return acc;

@@ -178,6 +178,23 @@ def test_what_an_adapter_holds_stays_with_its_rows(_sampler_session):
     one.check(one.run(s))
 
 
+def test_a_projection_of_nothing_but_nan(_sampler_session):
+    """Weights, then hidden states of NaN and infinities throughout: every logit is worked out again or known to be NaN, in no time
+    to speak of."""
+    import torch
+    s = _sampler_session
+    c = _Case(torch, 11, 256, 6000, 256, 8, 16)
+    inf, nan = f32_to_bf16_bits(np.float32([np.inf, np.nan]))
+    w = c.w.copy()
+    c.w[:, -1] = nan
+    c.upload()
+    assert np.isnan(c.run(s)).all()
+    c.w = w
+    c.x[:, ::2], c.x[:, 1::2] = inf, inf | np.uint16(0x8000)
+    c.upload()
+    c.check(c.run(s))
+
+
 def test_the_same_call_gives_the_same_bits_and_two_graphs_run_at_once(_sampler_session):
     import torch
     s = _sampler_session
