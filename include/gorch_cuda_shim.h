@@ -415,7 +415,8 @@ int gorch_cuda_cross_entropy_bwd_dev(GorchCudaCtxRef ctx, const void* logits, in
  * gorch_cuda_distill_fwd_dev: row_loss[b] = T^2 sum_i p_i (log p_i - log q_i); mean_loss[0] = sum(row_loss) / B
  * (may be NULL); row_stats [B][4] = (M, S, tM, tS), M = max x, S = sum exp((x - M) / T), tM and tS the same of
  * the entries: what the backward pass needs. A row without entries (padding): loss 0, stats 0, and
- * its logits are not read. A token listed twice counts as two entries.
+ * its logits are not read. A token listed twice counts as two entries (the backward pass then compares
+ * the row's entries with one another, which takes its time where k is in the thousands).
  * gorch_cuda_distill_bwd_dev: dx[b,j] = scale * row_grads[b] * T * (q_j - p of token j), f32 [B,dx_stride];
  * row_grads may be NULL (1); accumulate != 0: added to what dx holds (rows without entries stay as
  * they are; otherwise they become 0), which puts this gradient on top of gorch_cuda_cross_entropy_bwd_dev's. dx may be
