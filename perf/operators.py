@@ -223,7 +223,7 @@ def prepare(case: dict, seed: int) -> dict:
         ad.b, ad.b_pitch, ad.b_stride = st["b"].data_ptr(), st["b"].stride(1), st["b"].stride(0)
         ad.scales, ad.n, ad.rank = st["scales"].data_ptr(), case["adapters"], case["rank"]
         st["adapters"] = ad
-        st["workspace"] = torch.empty(s.lm_head_adapters_workspace(B, case["hidden"], ad), device="cuda", dtype=torch.uint8)
+        st["workspace"] = torch.empty(s.lm_head_adapters_workspace(B, ad), device="cuda", dtype=torch.uint8)
     return st
 
 
