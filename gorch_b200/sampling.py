@@ -410,8 +410,14 @@ class CudaSampler:
         rc = self._lib.gorch_cuda_lm_head_logits_dev(self._ctx, x_ptr, ldx, w_ptr, ldw, B, V, K, out_ptr, ld_out, C.byref(err))
         _check(self._lib, rc, err)
 
-    def lm_head_adapters_workspace(self, B: int, K: int, adapters) -> int:
-        """gorch_cuda_lm_head_adapters_workspace: bytes of device memory that lm_head_adapters_ptrs needs for B rows of K."""
+    def lm_head_adapters_workspace(self, B: int, K, adapters=None) -> int:
+        """gorch_cuda_lm_head_adapters_workspace: bytes of device memory that lm_head_adapters_ptrs needs for B rows of K
+        (`adapters`: a _lib.Adapters record). Without K, as lm_head_adapters_workspace(B, adapters), it is room for the widest
+        rows that the record's a_pitch holds, and so for any."""
+        if K is None or isinstance(K, _lib.Adapters):
+            if adapters is not None:
+                raise TypeError("lm_head_adapters_workspace takes (B, K, adapters) or (B, adapters)")
+            K, adapters = 0 if K is None else K.a_pitch // 64 * 64, K
         n, err = C.c_uint64(0), C.c_void_p()
         rc = self._lib.gorch_cuda_lm_head_adapters_workspace(B, K, C.byref(adapters) if adapters is not None else None, C.byref(n), C.byref(err))
         _check(self._lib, rc, err)
