@@ -123,7 +123,8 @@ int gorch_cuda_set_kernel_variant(GorchCudaCtxRef ctx, int variant, int cluster_
 
 /* ---- device buffers: replaces metal_create_shared_buffer /
  * metal_buffer_contents / metal_release_buffer (metal/shim.h:21-28). CUDA
- * memory is not host-visible, so contents move by upload/download. ---- */
+ * memory is not host-visible, so contents move by upload/download. An upload is on the device when the call
+ * returns, for work on any stream; a download does not wait for the context's stream (gorch_cuda_sync). ---- */
 GorchCudaBufferRef gorch_cuda_buffer_alloc(GorchCudaCtxRef ctx, uint64_t bytes, char** errOut);
 void gorch_cuda_buffer_free(GorchCudaBufferRef buf);
 uint64_t gorch_cuda_buffer_length(GorchCudaBufferRef buf);
