@@ -191,7 +191,9 @@ __global__ void __launch_bounds__(DF_NT, DF_PER_SM) distill_fwd_kernel(const __g
   if (warp_teaches) {
     const double d = static_cast<double>(tm) - static_cast<double>(tM);
     const double f = ts == 0.0 ? 0.0 : static_cast<double>(expf(static_cast<float>(d / static_cast<double>(A.T))));
-    if (f == 0.0) { ts = 0.0; at = 0.0; ax = 0.0; } else { at = f * (at + ts * d); ax *= f; ts *= f; }
+    if (ts == ts) {                                            // (a NaN stays: with nothing else among the thread's entries there is no maximum, and f = 0)
+      if (f == 0.0) { ts = 0.0; at = 0.0; ax = 0.0; } else { at = f * (at + ts * d); ax *= f; ts *= f; }
+    }
     ts = warp_sum_d(ts); at = warp_sum_d(at); ax = warp_sum_d(ax);
   }
   if (lane == 0) { s_sum[0][warp] = sum; s_sum[1][warp] = warp_teaches ? ts : 0.0; s_sum[2][warp] = warp_teaches ? at : 0.0; s_sum[3][warp] = warp_teaches ? ax : 0.0; }

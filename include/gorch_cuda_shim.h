@@ -422,8 +422,9 @@ int gorch_cuda_cross_entropy_bwd_dev(GorchCudaCtxRef ctx, const void* logits, in
  * row_grads may be NULL (1); accumulate != 0: added to what dx holds (rows without entries stay as
  * they are; otherwise they become 0), which puts this gradient on top of gorch_cuda_cross_entropy_bwd_dev's. dx may be
  * the logits themselves if those are f32 with the same stride (accumulate 0), and must not overlap them otherwise.
- * The temperature lies in 1e-6 .. 1e6. NaN, +Inf or nothing but -Inf in a taught row makes its loss and gradient
- * NaN; an entry whose logit in x is -Inf makes the loss +Inf, and the gradient stays finite. */
+ * The temperature lies in 1e-6 .. 1e6. NaN, +Inf or nothing but -Inf in a taught row of x makes its loss and gradient
+ * NaN; NaN or +Inf among its entries makes its loss NaN, and its gradient at the listed tokens (all of them). An entry
+ * whose logit in x is -Inf makes the loss +Inf, and the gradient stays finite. */
 int gorch_cuda_distill_fwd_dev(GorchCudaCtxRef ctx, const void* logits, int dtype, int64_t B, int64_t V,
                                int64_t row_stride, const int32_t* teacher_ids, const float* teacher_logits,
                                int64_t k, int64_t teacher_stride, float temperature, float* row_loss,
