@@ -1469,8 +1469,11 @@ static int check_generate_control(const int32_t* ids, const GorchGenControl* gc,
   return GORCH_CUDA_OK;
 }
 
+// The mask that a step's logits went through, and the logits themselves.
+struct MaskedStep { const GorchLogitAdjust* adj; const void* logits; int dtype; int64_t V, row_stride; int32_t* out_ids; };
+
 static int launch_generate_control(Ctx* c, const int32_t* ids, const uint32_t* flags,
-                                   const GorchGenControl* gc, int64_t B, char** errOut, const GorchLogitAdjust* adj = nullptr) {
+                                   const GorchGenControl* gc, int64_t B, char** errOut, const MaskedStep* masked = nullptr) {
   const int rc = check_generate_control(ids, gc, B, errOut);
   if (rc || B == 0) return rc;
   gs::GenControlArgs a{};
@@ -1482,8 +1485,12 @@ static int launch_generate_control(Ctx* c, const int32_t* ids, const uint32_t* f
   a.n_stop = gc->n_stop; a.max_new = gc->max_new; a.max_seq = gc->max_seq; a.cached = gc->cached ? 1 : 0;
   a.bad_flags = GORCH_FLAG_INTERNAL | GORCH_FLAG_BAD_CFG;
   a.B = static_cast<int>(B);
-  if (adj && adj->mask) {                                    // (ids are below V, which the mask covers)
+  if (masked && masked->adj->mask) {                         // (ids are below V, which the mask covers)
+    const GorchLogitAdjust* adj = masked->adj;
     a.mask = adj->mask; a.mask_stride = adj->mask_stride; a.n_masks = static_cast<int>(adj->n_masks); a.mask_rows = adj->mask_rows;
+    a.logits = masked->logits; a.row_stride = masked->row_stride; a.V = static_cast<int>(masked->V);
+    a.bf16 = masked->dtype == GORCH_CUDA_BF16 ? 1 : 0;
+    a.out_ids = masked->out_ids;
   }
   CUDA_TRY(launch(c, gs::generate_control_kernel, 1, gs::GC_NT, 0, true, a), errOut);
   c->counters.kernel_launches += 1;
@@ -1680,7 +1687,8 @@ int gorch_cuda_generate_step_adjusted_dev(GorchCudaCtxRef ctx, void* logits, int
   if ((rc = launch_adjust(c, logits, dtype, B, V, row_stride, adjust, logits, row_stride, gc, errOut))) return rc;
   rc = launch_rows(c, logits, dtype, B, V, row_stride, cfgs, uniforms, out_ids, out_flags, nullptr, nullptr, 0, errOut, nullptr, gc->done);
   if (rc) return rc;
-  return launch_generate_control(c, out_ids, out_flags, gc, B, errOut, adjust);
+  const MaskedStep masked{adjust, logits, dtype, V, row_stride, out_ids};
+  return launch_generate_control(c, out_ids, out_flags, gc, B, errOut, &masked);
 }
 
 // CTAs per row of the resident softmax: as few as leave room for two slices per SM (any number up to eight), twice as many

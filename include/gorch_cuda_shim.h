@@ -376,8 +376,11 @@ int gorch_cuda_adjust_logits_dev(GorchCudaCtxRef ctx, const void* logits, int dt
 /* gorch_cuda_generate_step_dev behind the rules: the logits of the live rows are adjusted in place, then
  * sampled, then the control step runs. The row's tokens are taken from the control record (gc->tokens,
  * gc->lengths; the last gc->n_new of them are the generated ones), and adjust's history fields are not
- * looked at. A sampled token that the row's mask does not allow (what the sampling calls return where the
- * mask leaves nothing) ends the row with GORCH_GEN_ERROR, nothing appended. */
+ * looked at. A row whose mask leaves nothing, or that cannot be sampled from (NaN, +Inf) and whose fallback token
+ * the mask does not allow, ends with GORCH_GEN_ERROR, nothing appended. Where the walk over any other row fell
+ * through (GORCH_FLAG_FALLBACK: rounding, with a uniform next to 1, or a mode A top_p that removes every token) to a
+ * V - 1 that the mask does not allow, the step takes the row's largest logit, the lowest index of equal ones, and
+ * out_ids says so. */
 int gorch_cuda_generate_step_adjusted_dev(GorchCudaCtxRef ctx, void* logits, int dtype, int64_t B,
                                           int64_t V, int64_t row_stride, const GorchLogitAdjust* adjust,
                                           const GorchSampleCfg* cfgs, const double* uniforms,
