@@ -105,25 +105,44 @@ struct LmHeadArgs {
 // faster: 276, 237). 64 rows with eight adapters of rank 16: 90 us (70 alone); one row: 70 (64).
 // So an adapter's b passes once per group, its products cost what its rows cost, rounded up to 32 (with every unit over all
 // rows of the item, 256 x 1,024 x 151,936 with 32 adapters of rank 32 took 290 us), and the epilogue's results are complete.
-// h goes in as two bf16, the rounded value and what the rounding left, each multiplied with the same tile of b: one bf16 would put
-// 2^-8 of the adapter's term on logits that are f32, two lose 2^-16 of it at most (the sums over K = 1,024, which the tensor pipe
-// cuts off rather than rounds, are off by 1.0e-6 of the logits' size by themselves, with the adapters 1.3e-6).
-// 0 times an Inf or NaN in an adapter's b is NaN, in the rows around its run too (and the two parts of h may disagree about an Inf in the
+// h goes in as three bf16, eight bits of the f32 value after eight, each multiplied with the same tile of b: nothing of h is lost.
+// The tensor pipe cuts its sums off where f32 would round them, which over K = 1,024 puts 1.0e-6 of the logits' size on them, and in
+// proportion to K. So they are cut into runs of LMA_SEG products, each with an accumulator of its own (the last goes on over
+// the adapters), and the epilogue adds those in registers, rounding to nearest. Errors as a share of the logits' size, root mean squares
+// against 64 bits, 64 rows, rank 16: K = 1,024: 4.9e-7 (one sum: 1.0e-6; an f32 product: 2.5e-7), K = 4,096: 4.7e-7 (4.4e-6; 5.9e-7); rank 256:
+// 8.0e-7. Runs of 256 halve it and cost more: one row 70 -> 76 us, 256 rows with 32 adapters of rank 32 236 -> 277.
+// 0 times an Inf or NaN in an adapter's b is NaN, in the rows around its run too (and the parts of h may disagree about an Inf in the
 // row's own): where a group has adapters, the epilogue works a NaN out again from the row's own operands, unless x holds one.
 constexpr int LMA_UNIT = 16;             // columns of the rank in a unit: K of one MMA, 32 bytes
+constexpr int LMA_PARTS = 3;             // bf16 that make up a value of h
+constexpr int LMA_SEG = 512;             // products of a sum on the tensor pipe
+// Of an item's nkc chunks of K, the first of the sum behind the one that begins with chunk kc. The last sum, which goes on over the
+// adapters, has fewer chunks where their rank is high, and the sums ahead of it what is left.
+__device__ __forceinline__ int lma_next_sum(int kc, int nkc, int units) {
+  constexpr int SEG = LMA_SEG / (LMH_SUB * LMH_BK), STEPS = LMH_SUB * LMH_BK / 16;   // chunks of a sum, steps of a chunk
+  const int last = nkc - max(1, min(SEG, SEG + (2 * STEPS - LMA_PARTS * units) / STEPS));
+  return kc >= last ? nkc : min(kc + SEG, last);
+}
 constexpr int LMA_STAGE = 4;             // units in a stage, and warps of a CTA that ask for them: one for each of a stage's units
-constexpr int LMA_RUN_NT = LMH_NT + 32 * LMA_STAGE;
+// Four warpgroups: producer and issuer (and two warps without work), two of the epilogue, those who ask for units. An epilogue thread holds the
+// sums of 128 logits, so the other warpgroups hand registers over to it, out of the 128 a thread that the block is launched with.
+constexpr int LMA_EPI0 = 4;              // the epilogue's first warp
+constexpr int LMA_RUN_NT = 512;
+constexpr int LMA_REGS_EPI = 176, LMA_REGS = 72, LMA_REGS_LAUNCH = 128;
+static_assert(LMA_EPI0 + LMH_EPI + LMA_STAGE == LMA_RUN_NT / 32 && 256 * LMA_REGS_EPI + 256 * LMA_REGS <= LMA_RUN_NT * LMA_REGS_LAUNCH, "what is handed over is there");
 constexpr int LMA_RING_BYTES = 200 * 1024, LMA_DYN_BYTES = LMA_RING_BYTES + 1024;
 constexpr int LMA_MAX_RANK = 256;
 constexpr int LMA_NT = 256;              // of the kernels ahead of the projection
 constexpr int LMA_BOX = 16;              // batch rows of h that one TMA load brings
-static_assert(LMA_STAGE * 2 * 32 <= LMH_SUB * LMH_BK * 2 && LMA_STAGE * LMH_CTA_V * 32 <= LMH_SUB * LMH_W_BYTES, "a stage holds its units");
-static_assert(LMA_NT >= LMH_MAX_N, "a thread per batch row of a group");
+// a stage's units: b in the first of w's boxes, two parts of h on the x side, the third in the second of w's boxes
+static_assert(LMA_PARTS == 3 && LMH_SUB == 2 && LMA_STAGE * 2 * 32 <= LMH_SUB * LMH_BK * 2 && LMA_STAGE * LMH_CTA_V * 32 <= LMH_W_BYTES &&
+              LMA_STAGE * (LMH_MAX_N / 2) * 32 <= LMH_W_BYTES, "a stage holds its units");
+static_assert(LMA_NT >= LMH_MAX_N && LMA_SEG % (LMH_SUB * LMH_BK) == 0, "a thread per batch row of a group, whole chunks in a sum");
 
 struct LmaRun { int32_t adapter, n0, n1, pad; };   // of a group: its rows n0 .. n1 - 1, multiples of 32, hold the adapter's
 struct LmAdaptArgs {
   CUtensorMap map_b;       // b [n, V, rank] bf16, box 16 x cta_v, 32-byte swizzle
-  CUtensorMap map_h;       // h [group][unit][2][item_n] rows of 16 bf16, box 16 x LMA_BOX, 32-byte swizzle
+  CUtensorMap map_h;       // h [group][unit][LMA_PARTS][item_n] rows of 16 bf16, box 16 x LMA_BOX, 32-byte swizzle
   const uint16_t *x, *w, *a, *b;
   int64_t ldx, ldw, a_pitch, a_stride, b_pitch, b_stride;   // in elements
   const float* scales;     // [n] or null: 1
@@ -141,7 +160,7 @@ struct LmAdaptArgs {
   uint16_t* h;
 };
 __device__ __forceinline__ int64_t lma_h_row(const LmAdaptArgs& D, int group, int unit, int piece, int row) {
-  return ((static_cast<int64_t>(group) * D.max_runs * D.units + unit) * 2 + piece) * D.item_n + row;
+  return ((static_cast<int64_t>(group) * D.max_runs * D.units + unit) * LMA_PARTS + piece) * D.item_n + row;
 }
 
 __device__ __forceinline__ float bf16_lo(uint32_t w) { return __uint_as_float(w << 16); }
@@ -178,7 +197,20 @@ __global__ void __launch_bounds__(LMA_NT) lm_adapters_order_kernel(const __grid_
   pdl_launch();
 }
 
-// A CTA per place of the order: the runs of its group, its row of x, its h. A batch of one group is put in order here (ordered == 0).
+// The next eight bits of v as a bf16, taken off v. Cut off, not rounded: a value next to f32's largest stays finite, and
+// 8 + 8 + 8 bits are all that f32 has. An infinity or a NaN is in the first part alone.
+__device__ __forceinline__ uint32_t lma_part(float& v) {
+  if (!(fabsf(v) < INFINITY)) {
+    const uint32_t bits = bf16_bits_rne(v);
+    v = 0.0f;
+    return bits;
+  }
+  const uint32_t top = __float_as_uint(v) & 0xffff0000u;
+  v -= __uint_as_float(top);                                         // (exact)
+  return top >> 16;
+}
+
+// A CTA per place of the order: the runs of its group, its row of x, its h. Up to LMA_NT rows are put in order here (ordered == 0).
 __global__ void __launch_bounds__(LMA_NT) lm_adapters_kernel(const __grid_constant__ LmAdaptArgs D, const int32_t ordered) {
   __shared__ __align__(16) int keys[4 * LMA_NT];
   __shared__ int s_ad[LMA_NT + 1], s_start[LMA_NT + 1], s_first[LMA_NT / 32], s_row, s_mine;
@@ -196,7 +228,7 @@ __global__ void __launch_bounds__(LMA_NT) lm_adapters_kernel(const __grid_consta
     s_ad[tid] = -1;
     const int place = lma_place(D, tid, a < 0 ? D.n : a, keys, tid);   // (its barriers come before the next line)
     if (tid < D.B) {
-      s_ad[place] = a;
+      if (place >= g0 && place < g0 + rows) s_ad[place - g0] = a;
       if (place == p) s_row = tid;
       if (p == 0) { D.order[place] = tid; D.sorted[place] = a; }
     }
@@ -256,31 +288,29 @@ __global__ void __launch_bounds__(LMA_NT) lm_adapters_kernel(const __grid_consta
   }
   const int any = __syncthreads_or(nan);                             // (and s_h and s_mine are there)
   if (tid == 0) D.row_nan[p] = any;
-  // 16 bytes at a time, half of a unit's row of either piece: this row of the runs whose 32s hold it
+  // this row of the runs whose 32s hold it: half of a unit's row at a time, 16 bytes of each part
   const int at = p - g0;
-  for (int i = tid; i < nruns * D.units * 4; i += LMA_NT) {
-    const int unit = i >> 2, piece = (i >> 1) & 1, half = i & 1, q = unit / D.units;
+  for (int i = tid; i < nruns * D.units * 2; i += LMA_NT) {
+    const int unit = i >> 1, half = i & 1, q = unit / D.units;
     if (at < (s_start[q] & ~31) || at >= ((s_start[q + 1] + 31) & ~31)) continue;
-    uint32_t o[4] = {0u, 0u, 0u, 0u};
+    uint32_t o[LMA_PARTS][4] = {};
     if (q == s_mine) {
       const int r0 = (unit - q * D.units) * LMA_UNIT + half * 8;
 #pragma unroll
       for (int c = 0; c < 8; c++) {
-        const float v = (r0 + c < D.rank) ? s_h[r0 + c] : 0.0f;
-        const uint32_t top = bf16_bits_rne(v);
-        const float left = v - __uint_as_float(top << 16);
-        // (an infinity's, and a NaN's, are in the rounded value)
-        const uint32_t bits = piece == 0 ? top : (fabsf(__uint_as_float(top << 16)) < INFINITY ? bf16_bits_rne(left) : 0u);
-        o[c >> 1] |= bits << (16 * (c & 1));
+        float v = (r0 + c < D.rank) ? s_h[r0 + c] : 0.0f;
+#pragma unroll
+        for (int piece = 0; piece < LMA_PARTS; piece++) o[piece][c >> 1] |= lma_part(v) << (16 * (c & 1));
       }
     }
-    uint4* dst = reinterpret_cast<uint4*>(D.h + lma_h_row(D, g, unit, piece, at) * LMA_UNIT) + half;
-    *dst = make_uint4(o[0], o[1], o[2], o[3]);
+#pragma unroll
+    for (int piece = 0; piece < LMA_PARTS; piece++)
+      *(reinterpret_cast<uint4*>(D.h + lma_h_row(D, g, unit, piece, at) * LMA_UNIT) + half) = make_uint4(o[piece][0], o[piece][1], o[piece][2], o[piece][3]);
   }
 }
 
 // One logit from its row's own operands, in f32; p: the row's place in the order.
-__device__ __noinline__ float lma_logit(const LmAdaptArgs& D, int p, int v) {
+__device__ __forceinline__ float lma_logit(const LmAdaptArgs& D, int p, int v) {
   const uint4 *x4 = reinterpret_cast<const uint4*>(D.xs + static_cast<int64_t>(p) * D.K), *w4 = reinterpret_cast<const uint4*>(D.w + v * D.ldw);
   float acc = 0.0f;
   for (int k = 0; k < D.K / 8; k++) {
@@ -298,9 +328,9 @@ __device__ __noinline__ float lma_logit(const LmAdaptArgs& D, int p, int v) {
   while (run < D.nruns[g] - 1 && runs[run].adapter != a) run++;
   const uint16_t* brow = D.b + a * D.b_stride + v * D.b_pitch;
   for (int r = 0; r < D.rank; r++) {
-    float h = 0.0f;                                                    // (the two parts' sum is exact)
+    float h = 0.0f;                                                    // (the parts' sum is exact)
 #pragma unroll
-    for (int piece = 0; piece < 2; piece++)
+    for (int piece = 0; piece < LMA_PARTS; piece++)
       h += __uint_as_float(static_cast<uint32_t>(D.h[lma_h_row(D, g, run * D.units + r / LMA_UNIT, piece, p - g * D.item_n) * LMA_UNIT + r % LMA_UNIT]) << 16);
     acc = fmaf(h, __uint_as_float(static_cast<uint32_t>(__ldg(brow + r)) << 16), acc);
   }
@@ -451,20 +481,63 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
       : "r"(taddr) : "memory");
 }
 
+// The items of an epilogue warp again, behind all its others: a lane reads back what it wrote. (Behind them, so that no wait is held up
+// by it, and where the sums' registers are free.)
+__device__ __noinline__ void lma_second_look(const LmHeadArgs& A, const LmAdaptArgs& D) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, q = warp & 3, half = (warp - LMA_EPI0) >> 2;
+  const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1, rank = blockIdx.x & 1;
+  const LmhPlan plan(A.B, A.ntile, A.item_n, npairs);
+  for (int i = pair; i < plan.total; i += npairs) {
+    const LmhItem it = plan.at(i);
+    if (D.nruns[it.b0 / A.item_n] == 0) continue;
+    const int in_tile = rank * A.cta_v + q * 32 + lane, v = (A.tile0 + it.vt * A.tile_step) * 2 * A.cta_v + in_tile;
+    const bool live = q * 32 + lane < A.cta_v && v < A.V;
+    for (int c = half * 32; c < it.n; c += 64) {
+      const int b0 = it.b0 + c, nb = min(32, A.B - b0);
+      for (int j = 0; j < nb; j++) {
+        if (D.row_nan[b0 + j]) continue;
+        float* at = A.out_logits + D.order[b0 + j] * A.ld_out + v;
+        if (live && *at != *at) *at = lma_logit(D, b0 + j, v);
+      }
+    }
+  }
+}
+
+// s += 16 columns of an accumulator, rounded to nearest. (One statement, so that 16 registers and no more hold what is loaded.)
+__device__ __forceinline__ void tmem_add16(uint32_t taddr, float* s) {
+  asm volatile(
+      "{\n\t.reg .b32 t<16>;\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {t0, t1, t2, t3, t4, t5, t6, t7, t8, t9, t10, t11, t12, t13, t14, t15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;\n\t"
+      "add.rn.f32 %0, %0, t0;\n\tadd.rn.f32 %1, %1, t1;\n\tadd.rn.f32 %2, %2, t2;\n\tadd.rn.f32 %3, %3, t3;\n\t"
+      "add.rn.f32 %4, %4, t4;\n\tadd.rn.f32 %5, %5, t5;\n\tadd.rn.f32 %6, %6, t6;\n\tadd.rn.f32 %7, %7, t7;\n\t"
+      "add.rn.f32 %8, %8, t8;\n\tadd.rn.f32 %9, %9, t9;\n\tadd.rn.f32 %10, %10, t10;\n\tadd.rn.f32 %11, %11, t11;\n\t"
+      "add.rn.f32 %12, %12, t12;\n\tadd.rn.f32 %13, %13, t13;\n\tadd.rn.f32 %14, %14, t14;\n\tadd.rn.f32 %15, %15, t15;\n\t}"
+      : "+f"(s[0]), "+f"(s[1]), "+f"(s[2]), "+f"(s[3]), "+f"(s[4]), "+f"(s[5]), "+f"(s[6]), "+f"(s[7]),
+        "+f"(s[8]), "+f"(s[9]), "+f"(s[10]), "+f"(s[11]), "+f"(s[12]), "+f"(s[13]), "+f"(s[14]), "+f"(s[15])
+      : "r"(taddr) : "memory");
+}
+
 // ADAPT: with D's adapters (D is null otherwise). It is then launched as a dependent of the kernel that puts the rows in order, with w
 // there before.
 template <bool ADAPT>
 __device__ __forceinline__ void lm_head_run(const LmHeadArgs& A, const LmAdaptArgs* D) {
+  // accumulators in tensor memory
+  constexpr int MAX_ACC = LMH_TMEM_COLS / (ADAPT ? LMH_MAX_N / 2 : LMH_MAX_N);
+  const int acc_cols = ADAPT && A.item_n <= LMH_MAX_N / 2 ? LMH_MAX_N / 2 : LMH_MAX_N;
+  const uint32_t nacc = static_cast<uint32_t>(LMH_TMEM_COLS / acc_cols);
   extern __shared__ __align__(16) unsigned char lmh_dyn[];
-  __shared__ __align__(8) unsigned long long full_bar[LMH_MAX_STAGES], empty_bar[LMH_MAX_STAGES], acc_full[2], acc_empty[2];
+  __shared__ __align__(8) unsigned long long full_bar[LMH_MAX_STAGES], empty_bar[LMH_MAX_STAGES], acc_full[MAX_ACC], acc_empty[MAX_ACC];
   __shared__ uint32_t tmem_base_s;
   __shared__ int abort_s;
   __shared__ __align__(16) float stash_thr[LMH_EPI][32];
   __shared__ uint2 stash[LMH_EPI][64];
   __shared__ int stash_row[LMH_EPI][64];
   __shared__ __align__(16) unsigned char lma_space[ADAPT ? (2 + LMA_STAGE) * sizeof(LmaTable) : 16];
+  __shared__ int lma_places[ADAPT ? LMH_EPI : 1][ADAPT ? LMH_MAX_N / 2 : 1];   // of an epilogue warp's batch rows: the rows' own places
   __shared__ uint32_t lma_given;                                        // stages of units that the producer has found free and announced
   LmaTable* lma_tables = reinterpret_cast<LmaTable*>(lma_space);     // warp 0's, warp 1's, and of those that ask for units
+  constexpr int EPI0 = ADAPT ? LMA_EPI0 : 2;                            // the epilogue's first warp
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t rank = blockIdx.x & 1u;                                // in the pair; 0 leads
   const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
@@ -482,7 +555,7 @@ __device__ __forceinline__ void lm_head_run(const LmHeadArgs& A, const LmAdaptAr
 
   if (tid == 0) {
     for (int s = 0; s < nst; s++) { mbar_init(smem_addr(&full_bar[s]), 1); mbar_init(smem_addr(&empty_bar[s]), 1); }
-    for (int b = 0; b < 2; b++) { mbar_init(smem_addr(&acc_full[b]), 1); mbar_init(smem_addr(&acc_empty[b]), 2 * LMH_EPI); }
+    for (int b = 0; b < MAX_ACC; b++) { mbar_init(smem_addr(&acc_full[b]), 1); mbar_init(smem_addr(&acc_empty[b]), 2 * LMH_EPI); }
     abort_s = 0;
     if constexpr (ADAPT) {
       for (int t = 0; t < 2 + LMA_STAGE; t++) lma_tables[t].group = -1;
@@ -500,6 +573,9 @@ __device__ __forceinline__ void lm_head_run(const LmHeadArgs& A, const LmAdaptAr
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem_base = tmem_base_s;
 
+  if constexpr (ADAPT) {
+    if (warp < EPI0 || warp >= EPI0 + LMH_EPI) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(LMA_REGS));
+  }
   if (warp == 0) {
     // ---- producer: this CTA's share of every stage; its bytes complete on the leader's barrier
     if (lane == 0) {
@@ -544,7 +620,7 @@ __device__ __forceinline__ void lm_head_run(const LmHeadArgs& A, const LmAdaptAr
           bool more = ok && un.next();
           while (more) {
             uint32_t bytes = 0;
-            for (int u = 0; u < LMA_STAGE && more; u++, more = un.next()) bytes += static_cast<uint32_t>(A.cta_v) * 32 + static_cast<uint32_t>(un.n1 - un.n0) * 32;
+            for (int u = 0; u < LMA_STAGE && more; u++, more = un.next()) bytes += static_cast<uint32_t>(A.cta_v) * 32 + static_cast<uint32_t>(un.n1 - un.n0) * (LMA_PARTS * 16);
             if (!mbar_wait(smem_addr(&empty_bar[stage]), phase ^ 1u, abort_flag)) { ok = false; break; }
             // (the pair's other CTA may have its copies there before this says how many there are: the phase waits for this arrival)
             if (rank == 0) mbar_expect_tx(smem_addr(&full_bar[stage]), 2 * bytes);
@@ -555,11 +631,11 @@ __device__ __forceinline__ void lm_head_run(const LmHeadArgs& A, const LmAdaptAr
         }
       }
     }
-  } else if (ADAPT && warp >= LMH_NT / 32) {
+  } else if (ADAPT && warp >= EPI0 + LMH_EPI) {
     // ---- who asks for the units: warp j for the j-th of every stage. (Which stages are free is the producer's word: one of these
     // could be rounds ahead of a barrier, and its parity would not say so.)
     if (lane == 0) {
-      const int j = warp - LMH_NT / 32;
+      const int j = warp - (EPI0 + LMH_EPI);
       unsigned long long pol_w, pol_x;
       asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(pol_w));
       asm volatile("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(pol_x));
@@ -592,6 +668,7 @@ __device__ __forceinline__ void lm_head_run(const LmHeadArgs& A, const LmAdaptAr
             for (int q = 0; q < half; q += LMA_BOX) {
               tma_load_2d_pair(sx + 2 * u * hb + q * 32, &D->map_h, bar, 0, hrow + q, pol_x);
               tma_load_2d_pair(sx + (2 * u + 1) * hb + q * 32, &D->map_h, bar, 0, hrow + A.item_n + q, pol_x);
+              tma_load_2d_pair(sw + LMH_W_BYTES + u * hb + q * 32, &D->map_h, bar, 0, hrow + 2 * A.item_n + q, pol_x);
             }
           }
           seen++;
@@ -608,8 +685,20 @@ __device__ __forceinline__ void lm_head_run(const LmHeadArgs& A, const LmAdaptAr
         const uint32_t idesc = lmh_idesc(plan.at(i).n);
         if (!mbar_wait(smem_addr(&acc_empty[acc]), acc_phase ^ 1u, abort_flag)) { ok = false; break; }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint32_t d_tmem = tmem_base + acc * LMH_MAX_N;
+        uint32_t d_tmem = tmem_base + acc * acc_cols;
+        int fresh = 0;                                                  // the chunk that begins a sum, and the one that begins the next
+        [[maybe_unused]] int next_sum = nkc;
+        if constexpr (ADAPT) next_sum = lma_next_sum(0, nkc, D->units);
         for (int kc = 0; kc < nkc; kc++) {
+          if (ADAPT && kc == next_sum) {                                // on to the next accumulator
+            umma_commit_pair(smem_addr(&acc_full[acc]));
+            if (++acc == nacc) { acc = 0; acc_phase ^= 1u; }
+            if (!mbar_wait(smem_addr(&acc_empty[acc]), acc_phase ^ 1u, abort_flag)) { ok = false; break; }
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            d_tmem = tmem_base + acc * acc_cols;
+            fresh = kc;
+            if constexpr (ADAPT) next_sum = lma_next_sum(kc, nkc, D->units);
+          }
           if (!mbar_wait(smem_addr(&full_bar[stage]), phase, abort_flag)) { ok = false; break; }
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
           const uint32_t sw = ring + stage * stage_bytes, sx = sw + LMH_SUB * LMH_W_BYTES;
@@ -617,7 +706,7 @@ __device__ __forceinline__ void lm_head_run(const LmHeadArgs& A, const LmAdaptAr
           for (int u = 0; u < subs; u++) {
 #pragma unroll
             for (int k = 0; k < LMH_BK / 16; k++)
-              umma_f16_pair(d_tmem, umma_desc(sw + u * LMH_W_BYTES + k * 32), umma_desc(sx + u * x_bytes + k * 32), idesc, (kc > 0 || u > 0 || k > 0) ? 1u : 0u);
+              umma_f16_pair(d_tmem, umma_desc(sw + u * LMH_W_BYTES + k * 32), umma_desc(sx + u * x_bytes + k * 32), idesc, (kc > fresh || u > 0 || k > 0) ? 1u : 0u);
           }
           umma_commit_pair(smem_addr(&empty_bar[stage]));               // the stage is free once these MMAs have read it
           if (++stage == static_cast<uint32_t>(nst)) { stage = 0; phase ^= 1u; }
@@ -632,29 +721,30 @@ __device__ __forceinline__ void lm_head_run(const LmHeadArgs& A, const LmAdaptAr
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t sw = ring + stage * stage_bytes, sx = sw + LMH_SUB * LMH_W_BYTES, hb = static_cast<uint32_t>(A.box_n) * 32;
             for (int u = 0; u < LMA_STAGE && more; u++, more = un.next()) {
-              for (int piece = 0; piece < 2; piece++)
-                umma_f16_pair(d_tmem + static_cast<uint32_t>(un.n0 - un.i0), umma_desc_32b(sw + u * (LMH_CTA_V * 32)), umma_desc_32b(sx + (2 * u + piece) * hb),
-                              lmh_idesc(un.n1 - un.n0), 1u);
+              for (int piece = 0; piece < LMA_PARTS; piece++)
+                umma_f16_pair(d_tmem + static_cast<uint32_t>(un.n0 - un.i0), umma_desc_32b(sw + u * (LMH_CTA_V * 32)),
+                              umma_desc_32b(piece < 2 ? sx + (2 * u + piece) * hb : sw + LMH_W_BYTES + u * hb), lmh_idesc(un.n1 - un.n0), 1u);
             }
             umma_commit_pair(smem_addr(&empty_bar[stage]));
             if (++stage == static_cast<uint32_t>(nst)) { stage = 0; phase ^= 1u; }
           }
         }
         if (ok) umma_commit_pair(smem_addr(&acc_full[acc]));            // the accumulator is complete
-        if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
+        if (++acc == nacc) { acc = 0; acc_phase ^= 1u; }
       }
     }
-  } else {
+  } else if (warp >= EPI0) {
+    if constexpr (ADAPT) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(LMA_REGS_EPI));
     // ---- epilogue: warp w reads TMEM lanes 32 * (w % 4) .. + 31; thread = vocabulary row
-    const int q = warp & 3, half = (warp - 2) >> 2;                     // this warp's lanes, and its share of the columns
+    const int q = warp & 3, half = (warp - EPI0) >> 2;                     // this warp's lanes, and its share of the columns
     uint32_t acc = 0, acc_phase = 0;
     bool ok = true;
     int nstash = 0;
     auto flush = [&](int count) {                                       // the stash's first `count` entries to their rows' lists
       __syncwarp();
       if (lane < count) {
-        const uint2 e = stash[warp - 2][lane];
-        const int b = stash_row[warp - 2][lane];
+        const uint2 e = stash[warp - EPI0][lane];
+        const int b = stash_row[warp - EPI0][lane];
         const float x = __uint_as_float(e.x);
         if (x != x) {
           atomicOr(&A.rows[b].nan, (e.y == 0u) ? 3 : 1);
@@ -665,48 +755,76 @@ __device__ __forceinline__ void lm_head_run(const LmHeadArgs& A, const LmAdaptAr
       }
       __syncwarp();
     };
+    [[maybe_unused]] int places_of = -1, places_n = 0;
+    [[maybe_unused]] bool adapted = false, saw_nan = false;
     if (A.chained) pdl_wait();                                          // the thresholds; tiles and MMAs are under way meanwhile
     for (int i = pair; i < plan.total && ok; i += npairs) {
       const LmhItem it = plan.at(i);
-      bool adapted = false;
-      if constexpr (ADAPT) adapted = D->nruns[it.b0 / A.item_n] > 0;
-      if (!mbar_wait(smem_addr(&acc_full[acc]), acc_phase, abort_flag)) { ok = false; break; }
-      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const int in_tile = static_cast<int>(rank) * A.cta_v + q * 32 + lane;
       const int v = (A.tile0 + it.vt * A.tile_step) * 2 * A.cta_v + in_tile;
       const bool live = q * 32 + lane < A.cta_v && v < A.V;
       const int ocol = A.compact ? it.vt * 2 * A.cta_v + in_tile : v;
+      const uint32_t lanes = tmem_base + (static_cast<uint32_t>(q * 32) << 16);
+      // the accumulator is free again: one arrival per epilogue warp of either CTA at the leader's barrier
+      auto give_back = [&]() {
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(map_rank(smem_addr(&acc_empty[acc]), 0));
+        if (++acc == nacc) { acc = 0; acc_phase ^= 1u; }
+      };
+      if constexpr (ADAPT) {
+        if (it.b0 != places_of || it.n != places_n) {                  // other batch rows than the last item's: a trip to L2
+          places_of = it.b0;
+          places_n = it.n;
+          adapted = D->nruns[it.b0 / A.item_n] > 0;
+          __syncwarp();
+          for (int c = half * 32; c < it.n; c += 64) lma_places[warp - EPI0][c / 64 * 32 + lane] = it.b0 + c + lane < A.B ? D->order[it.b0 + c + lane] : 0;
+          __syncwarp();
+        }
+        auto finish = [&](float (&sum)[32], int c) {                   // the logits of 32 batch rows to their rows' places
+          const int b0 = it.b0 + c, nb = min(32, A.B - b0);            // (uniform)
+          if (adapted && live) {
+#pragma unroll
+            for (int j = 0; j < 32; j++) saw_nan |= sum[j] != sum[j] && j < nb;
+          }
+#pragma unroll
+          for (int j = 0; j < 32; j++) {
+            const int64_t to = lma_places[warp - EPI0][c / 64 * 32 + j];
+            if (j < nb && live) __stcs(A.out_logits + to * A.ld_out + ocol, sum[j]);
+            if (j % 8 == 7) asm volatile("" ::: "memory");             // (else 32 addresses at a time, and no registers left)
+          }
+        };
+        constexpr int CHUNKS = LMH_MAX_N / 64;                         // of 32 batch rows that a warp has
+        float sum[CHUNKS][32] = {};
+        for (int kc = 0; kc < nkc && ok; kc = lma_next_sum(kc, nkc, D->units)) {                  // an item's sums, added up as they come
+          if (!mbar_wait(smem_addr(&acc_full[acc]), acc_phase, abort_flag)) { ok = false; break; }
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+          for (int ch = 0; ch < CHUNKS; ch++) {
+            const int c = half * 32 + ch * 64;
+            if (c >= it.n) break;                                      // (uniform)
+            tmem_add16(lanes + acc * acc_cols + c, sum[ch]);
+            tmem_add16(lanes + acc * acc_cols + c + 16, sum[ch] + 16);
+          }
+          give_back();
+        }
+        if (!ok) break;
+#pragma unroll
+        for (int ch = 0; ch < CHUNKS; ch++) {
+          const int c = half * 32 + ch * 64;
+          if (c < it.n) finish(sum[ch], c);
+        }
+        continue;
+      }
+      if (!mbar_wait(smem_addr(&acc_full[acc]), acc_phase, abort_flag)) { ok = false; break; }
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
       for (int c = half * 32; c < it.n; c += 64) {
         uint32_t r[32];
-        tmem_ld32(tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * LMH_MAX_N + c, r);
+        tmem_ld32(lanes + acc * acc_cols + c, r);
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
         const int b0 = it.b0 + c, nb = min(32, A.B - b0);              // batch rows of these columns (uniform)
-        if constexpr (ADAPT) {
-          if (adapted) {
-            uint32_t bad = 0u;
-#pragma unroll
-            for (int j = 0; j < 32; j++) bad |= (__uint_as_float(r[j]) != __uint_as_float(r[j])) ? 1u << j : 0u;
-            if (bad != 0u && live) {
-#pragma unroll 1
-              for (int j = 0; j < nb; j++) {
-                if (!((bad >> j) & 1u) || D->row_nan[b0 + j]) continue;
-                const uint32_t y = __float_as_uint(lma_logit(*D, b0 + j, v));
-#pragma unroll
-                for (int jj = 0; jj < 32; jj++) r[jj] = (j == jj) ? y : r[jj];
-              }
-            }
-            __syncwarp();
-          }
-        }
-        if constexpr (ADAPT) {                                         // to the rows' own places
-          const int mine = lane < nb ? D->order[b0 + lane] : 0;
-#pragma unroll
-          for (int j = 0; j < 32; j++) {
-            const int64_t to = __shfl_sync(FULL, mine, j);
-            if (j < nb && live) __stcs(A.out_logits + to * A.ld_out + ocol, __uint_as_float(r[j]));
-          }
-        } else if (A.out_logits && live) {
+        if (A.out_logits && live) {
           float* dst = A.out_logits + static_cast<int64_t>(b0) * A.ld_out + ocol;
           if (nb == 32) {
 #pragma unroll
@@ -720,9 +838,9 @@ __device__ __forceinline__ void lm_head_run(const LmHeadArgs& A, const LmAdaptAr
           // a batch row's threshold is the same for all lanes, and few lanes hold a logit that reaches it: those go to
           // the warp's stash, and from there, 32 at a time, to their rows' lists (an atomic on a row's count per
           // logit where it is found made every warp wait in nearly every chunk)
-          stash_thr[warp - 2][lane] = (lane < nb) ? A.thr[b0 + lane] : INFINITY;
+          stash_thr[warp - EPI0][lane] = (lane < nb) ? A.thr[b0 + lane] : INFINITY;
           __syncwarp();
-          const float4* t4 = reinterpret_cast<const float4*>(stash_thr[warp - 2]);
+          const float4* t4 = reinterpret_cast<const float4*>(stash_thr[warp - EPI0]);
           uint32_t m = 0u;                                             // columns of this lane that reach their threshold
 #pragma unroll
           for (int j = 0; j < 32; j++) {
@@ -739,29 +857,29 @@ __device__ __forceinline__ void lm_head_run(const LmHeadArgs& A, const LmAdaptAr
 #pragma unroll
               for (int jj = 1; jj < 32; jj++) x = (j == jj) ? r[jj] : x;
               const int at = nstash + __popc(votes & ((1u << lane) - 1u));
-              stash[warp - 2][at] = make_uint2(x, static_cast<uint32_t>(v));
-              stash_row[warp - 2][at] = b0 + j;
+              stash[warp - EPI0][at] = make_uint2(x, static_cast<uint32_t>(v));
+              stash_row[warp - EPI0][at] = b0 + j;
             }
             nstash += __popc(votes);
             if (nstash >= 32) {                                        // uniform
               flush(32);
               nstash -= 32;
-              const uint2 e = stash[warp - 2][32 + lane];
-              const int er = stash_row[warp - 2][32 + lane];
+              const uint2 e = stash[warp - EPI0][32 + lane];
+              const int er = stash_row[warp - EPI0][32 + lane];
               __syncwarp();
-              if (lane < nstash) { stash[warp - 2][lane] = e; stash_row[warp - 2][lane] = er; }
+              if (lane < nstash) { stash[warp - EPI0][lane] = e; stash_row[warp - EPI0][lane] = er; }
             }
           }
           __syncwarp();
         }
       }
-      // the accumulator is free again: one arrival per epilogue warp of either CTA at the leader's barrier
-      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(map_rank(smem_addr(&acc_empty[acc]), 0));
-      if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
+      give_back();
     }
     if (nstash > 0) flush(nstash);
+    if constexpr (ADAPT) {                                              // the NaNs among what this warp wrote, once more
+      if (__any_sync(FULL, saw_nan)) lma_second_look(A, *D);
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(LMA_REGS));   // (as the warps have that it meets again)
+    }
   }
   // ---- teardown
   __syncwarp();

@@ -873,6 +873,10 @@ GorchCudaCtxRef gorch_cuda_create_ctx(int device, char** errOut) {
   if ((e = cudaFuncSetAttribute(gs::w1024::wide_rows_kernel<uint16_t>, cudaFuncAttributeMaxDynamicSharedMemorySize, gs::w1024::W_DYN_BYTES)) != cudaSuccess) return fail("cudaFuncSetAttribute", e);
   if ((e = cudaFuncSetAttribute(gs::lm_head_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, gs::LMH_DYN_BYTES)) != cudaSuccess) return fail("cudaFuncSetAttribute", e);
   if ((e = cudaFuncSetAttribute(gs::lm_head_adapters_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, gs::LMA_DYN_BYTES)) != cudaSuccess) return fail("cudaFuncSetAttribute", e);
+  // (the registers that its warpgroups hand over have to be the block's, or the ones that ask for them would wait for good)
+  cudaFuncAttributes adapters_kernel;
+  if ((e = cudaFuncGetAttributes(&adapters_kernel, gs::lm_head_adapters_kernel)) != cudaSuccess) return fail("cudaFuncGetAttributes", e);
+  if (adapters_kernel.numRegs < gs::LMA_REGS_LAUNCH) return fail("lm_head_adapters_kernel built for fewer registers than its warpgroups share", cudaErrorInvalidKernelImage);
   if ((e = cudaFuncSetAttribute(gs::lmh_finish_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, gs::LMH_F_DYN_BYTES)) != cudaSuccess) return fail("cudaFuncSetAttribute", e);
   if ((e = cudaFuncSetAttribute(gs::row_softmax_kernel<float>, cudaFuncAttributeMaxDynamicSharedMemorySize, gs::RS_DYN_BYTES)) != cudaSuccess) return fail("cudaFuncSetAttribute", e);
   if ((e = cudaFuncSetAttribute(gs::row_softmax_kernel<uint16_t>, cudaFuncAttributeMaxDynamicSharedMemorySize, gs::RS_DYN_BYTES)) != cudaSuccess) return fail("cudaFuncSetAttribute", e);
@@ -1967,7 +1971,7 @@ static AdapterSpace adapter_space(int64_t B, int64_t K, const GorchAdapters* ad)
   s.off_sorted = take(B * 4);
   s.off_nan = take(B * 4);
   s.off_x = take(B * K * 2);
-  s.off_h = take(s.groups * s.max_runs * s.units * 2 * s.item_n * gs::LMA_UNIT * 2);
+  s.off_h = take(s.groups * s.max_runs * s.units * gs::LMA_PARTS * s.item_n * gs::LMA_UNIT * 2);
   s.bytes = at;
   return s;
 }
@@ -2023,7 +2027,7 @@ int gorch_cuda_lm_head_adapters_dev(GorchCudaCtxRef ctx, const void* x, int64_t 
     set_err(errOut, "gorch_cuda: workspace of %llu bytes, %lld needed", (unsigned long long)workspace_bytes, (long long)sp.bytes);
     return GORCH_CUDA_ERR_BAD_ARG;
   }
-  const int64_t h_rows = sp.groups * sp.max_runs * sp.units * 2 * sp.item_n;
+  const int64_t h_rows = sp.groups * sp.max_runs * sp.units * gs::LMA_PARTS * sp.item_n;
   if (h_rows > 0x7fffffffll) { set_err(errOut, "gorch_cuda: more adapters and batch rows than 31 bits of workspace rows hold"); return GORCH_CUDA_ERR_LIMIT; }
   CUDA_TRY(cudaSetDevice(c->device), errOut);
   if ((rc = load_encode_tiled(errOut))) return rc;
@@ -2055,7 +2059,7 @@ int gorch_cuda_lm_head_adapters_dev(GorchCudaCtxRef ctx, const void* x, int64_t 
   if ((rc = make_unit_map(&d.map_b, adapters->b, adapters->rank, V, adapters->b_pitch, adapters->n, d.b_stride, a.cta_v, errOut))) return rc;
   if ((rc = make_unit_map(&d.map_h, d.h, gs::LMA_UNIT, h_rows, gs::LMA_UNIT, 0, 0, gs::LMA_BOX, errOut))) return rc;
   // The first kernel is no dependent: the projection reads w, and the second x, without a wait for what came before the call.
-  const bool several = sp.groups > 1;
+  const bool several = B > gs::LMA_NT;
   if (several) {
     CUDA_TRY(launch(c, gs::lm_adapters_order_kernel, static_cast<unsigned>((B + gs::LMA_NT - 1) / gs::LMA_NT), gs::LMA_NT, 0, false, d), errOut);
     c->counters.kernel_launches += 1;

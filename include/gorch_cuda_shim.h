@@ -453,8 +453,10 @@ int gorch_cuda_lm_head_status(GorchCudaCtxRef ctx, uint32_t* status, char** errO
  * projection is the plain MatMulTransB above):
  *   logits[b, v] = sum_k x[b, k] w[v, k] + scales[i] sum_r b[i, v, r] (sum_k a[i, r, k] x[b, k]),   i = row_adapter[b]
  * in one pass over the weights, whatever adapters the rows of a batch have; a row whose row_adapter lies
- * outside [0, n) (-1) gets the projection alone. a and b are bf16, sums are f32, and the inner product with a is handed on in two
- * bf16 (it loses 2^-16 at most). What one row's adapter holds does not reach other rows, infinities and NaN
+ * outside [0, n) (-1) gets the projection alone. a and b are bf16, sums and the inner product with a are f32. (The tensor
+ * cores cut sums off where f32 rounds; here in sums of 512 products, which are then added up, where
+ * gorch_cuda_lm_head_logits_dev has one over all of K: for rows without an adapter the two agree bit for bit up to K = 512
+ * and rank 112, and this one is the more exact beyond.) What one row's adapter holds does not reach other rows, infinities and NaN
  * included. Operands as for gorch_cuda_lm_head_logits_dev; a and b 16-byte aligned, pitches and strides multiples of 8
  * elements; rank 1 .. 256. The workspace (device memory of the size that gorch_cuda_lm_head_adapters_workspace
  * gives, 256-byte aligned) is the call's while it runs: calls that may overlap, captured ones among them,
