@@ -309,32 +309,35 @@ __global__ void __launch_bounds__(LMA_NT) lm_adapters_kernel(const __grid_consta
   }
 }
 
-// One logit from its row's own operands, in f32; p: the row's place in the order.
-__device__ __forceinline__ float lma_logit(const LmAdaptArgs& D, int p, int v) {
+// One logit from its row's own operands, in f32. p: the row's place in the order; a: its adapter (below 0: none), run: that one's in its
+// group. The adapter's part first: a NaN there settles it at little cost.
+__device__ __forceinline__ float lma_logit(const LmAdaptArgs& D, int p, int v, int a, int run) {
+  float own = 0.0f;
+  if (a >= 0) {
+    const int g = p / D.item_n;
+    const uint16_t* brow = D.b + a * D.b_stride + v * D.b_pitch;
+    for (int r = 0; r < D.rank && own == own; r++) {
+      float h = 0.0f;                                                    // (the parts' sum is exact)
+#pragma unroll
+      for (int piece = 0; piece < LMA_PARTS; piece++)
+        h += __uint_as_float(static_cast<uint32_t>(D.h[lma_h_row(D, g, run * D.units + r / LMA_UNIT, piece, p - g * D.item_n) * LMA_UNIT + r % LMA_UNIT]) << 16);
+      own = fmaf(h, __uint_as_float(static_cast<uint32_t>(__ldg(brow + r)) << 16), own);
+    }
+  }
   const uint4 *x4 = reinterpret_cast<const uint4*>(D.xs + static_cast<int64_t>(p) * D.K), *w4 = reinterpret_cast<const uint4*>(D.w + v * D.ldw);
   float acc = 0.0f;
-  for (int k = 0; k < D.K / 8; k++) {
-    const uint4 q = x4[k], t = __ldg(w4 + k);
-    const uint32_t qs[4] = {q.x, q.y, q.z, q.w}, ts[4] = {t.x, t.y, t.z, t.w};
+  for (int k0 = 0; k0 < D.K / 8 && own == own && acc == acc; k0 += LMH_BK / 8) {
+    uint4 q[LMH_BK / 8], t[LMH_BK / 8];
 #pragma unroll
-    for (int c = 0; c < 4; c++) { acc = fmaf(bf16_lo(qs[c]), bf16_lo(ts[c]), acc); acc = fmaf(bf16_hi(qs[c]), bf16_hi(ts[c]), acc); }
-    if (acc != acc) return acc;                                        // (a NaN of the projection's own)
-  }
-  const int a = D.sorted[p];
-  if (a < 0) return acc;
-  const int g = p / D.item_n;
-  const LmaRun* runs = D.runs + static_cast<int64_t>(g) * D.max_runs;
-  int run = 0;
-  while (run < D.nruns[g] - 1 && runs[run].adapter != a) run++;
-  const uint16_t* brow = D.b + a * D.b_stride + v * D.b_pitch;
-  for (int r = 0; r < D.rank; r++) {
-    float h = 0.0f;                                                    // (the parts' sum is exact)
+    for (int k = 0; k < LMH_BK / 8; k++) { q[k] = x4[k0 + k]; t[k] = __ldg(w4 + k0 + k); }
 #pragma unroll
-    for (int piece = 0; piece < LMA_PARTS; piece++)
-      h += __uint_as_float(static_cast<uint32_t>(D.h[lma_h_row(D, g, run * D.units + r / LMA_UNIT, piece, p - g * D.item_n) * LMA_UNIT + r % LMA_UNIT]) << 16);
-    acc = fmaf(h, __uint_as_float(static_cast<uint32_t>(__ldg(brow + r)) << 16), acc);
+    for (int k = 0; k < LMH_BK / 8; k++) {
+      const uint32_t qs[4] = {q[k].x, q[k].y, q[k].z, q[k].w}, ts[4] = {t[k].x, t[k].y, t[k].z, t[k].w};
+#pragma unroll
+      for (int c = 0; c < 4; c++) { acc = fmaf(bf16_lo(qs[c]), bf16_lo(ts[c]), acc); acc = fmaf(bf16_hi(qs[c]), bf16_hi(ts[c]), acc); }
+    }
   }
-  return acc;
+  return acc + own;
 }
 
 // A group's runs in shared memory, one table for each of the threads that walk them: a trip to L2 for every run of every
@@ -489,7 +492,9 @@ __device__ __noinline__ void lma_second_look(const LmHeadArgs& A, const LmAdaptA
   const LmhPlan plan(A.B, A.ntile, A.item_n, npairs);
   for (int i = pair; i < plan.total; i += npairs) {
     const LmhItem it = plan.at(i);
-    if (D.nruns[it.b0 / A.item_n] == 0) continue;
+    const int nruns = D.nruns[it.b0 / A.item_n];
+    if (nruns == 0) continue;
+    const LmaRun* runs = D.runs + static_cast<int64_t>(it.b0 / A.item_n) * D.max_runs;
     const int in_tile = rank * A.cta_v + q * 32 + lane, v = (A.tile0 + it.vt * A.tile_step) * 2 * A.cta_v + in_tile;
     const bool live = q * 32 + lane < A.cta_v && v < A.V;
     for (int c = half * 32; c < it.n; c += 64) {
@@ -497,7 +502,15 @@ __device__ __noinline__ void lma_second_look(const LmHeadArgs& A, const LmAdaptA
       for (int j = 0; j < nb; j++) {
         if (D.row_nan[b0 + j]) continue;
         float* at = A.out_logits + D.order[b0 + j] * A.ld_out + v;
-        if (live && *at != *at) *at = lma_logit(D, b0 + j, v);
+        const bool odd = live && *at != *at;
+        if (!__any_sync(FULL, odd)) continue;
+        const int a = D.sorted[b0 + j];
+        int run = -1;
+        for (int r0 = 0; a >= 0 && run < 0; r0 += 32) {                  // (it is there)
+          const uint32_t hit = __ballot_sync(FULL, r0 + lane < nruns && runs[r0 + lane].adapter == a);
+          if (hit != 0u || r0 + 32 >= nruns) run = r0 + max(__ffs(hit) - 1, 0);
+        }
+        if (odd) *at = lma_logit(D, b0 + j, v, a, run);
       }
     }
   }

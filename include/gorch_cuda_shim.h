@@ -457,7 +457,8 @@ int gorch_cuda_lm_head_status(GorchCudaCtxRef ctx, uint32_t* status, char** errO
  * cores cut sums off where f32 rounds; here in sums of 512 products, which are then added up, where
  * gorch_cuda_lm_head_logits_dev has one over all of K: for rows without an adapter the two agree bit for bit up to K = 512
  * and rank 112, and this one is the more exact beyond.) What one row's adapter holds does not reach other rows, infinities and NaN
- * included. Operands as for gorch_cuda_lm_head_logits_dev; a and b 16-byte aligned, pitches and strides multiples of 8
+ * included (rows next to those of an adapter that holds some are worked out again, and the call takes up to 40 times as long).
+ * Operands as for gorch_cuda_lm_head_logits_dev; a and b 16-byte aligned, pitches and strides multiples of 8
  * elements; rank 1 .. 256. The workspace (device memory of the size that gorch_cuda_lm_head_adapters_workspace
  * gives, 256-byte aligned) is the call's while it runs: calls that may overlap, captured ones among them,
  * each need their own. Asynchronous; gorch_cuda_lm_head_status covers it. */
