@@ -123,8 +123,8 @@ class DeviceGenerateState:
         their history (gorch_cuda_generate_step_adjusted_dev)."""
         err = C.c_void_p()
         if rules is not None:
-            if getattr(rules, "B", self.B) != self.B:
-                raise ValueError("the rules are of another batch size")
+            if hasattr(rules, "check"):
+                rules.check(self.B, V)
             rc = self.s._lib.gorch_cuda_generate_step_adjusted_dev(
                 self.s._ctx, logits_ptr, dtype, self.B, V, row_stride, C.byref(getattr(rules, "record", rules)), cfgs_ptr,
                 uniforms_ptr, self.ids_ptr, self.flags_ptr, C.byref(self.gc), C.byref(err))

@@ -38,6 +38,7 @@ class LogitRules:
     def __init__(self, sampler: CudaSampler, B: int, penalties=None, history=None, prompt_lengths=None, bias=None, masks=None,
                  mask_rows=None):
         parts, rec = [], _lib.LogitAdjust()
+        self.V = None                                                 # the vocabulary, where the masks say it
 
         def add(field, arr):
             parts.append((field, arr))
@@ -83,7 +84,11 @@ class LogitRules:
             rec.n_bias = len(flat)
         if masks is not None:
             words = np.asarray(masks)
-            words = np.ascontiguousarray(words) if words.dtype == np.uint32 else pack_masks(words)
+            if words.dtype == np.uint32:
+                words = np.ascontiguousarray(words)
+            else:
+                words = pack_masks(words)
+                self.V = np.shape(masks)[1]
             if words.ndim != 2:
                 raise ValueError("masks must be [n, V] truth values or [n, words] uint32")
             add("mask", words)
@@ -109,6 +114,14 @@ class LogitRules:
         for field, _, o in places:
             setattr(rec, field, base + o)
 
+    def check(self, B: int, V: int) -> None:
+        """Refuses logits [B, V] that these rules are not for. (Masks of truth values for fewer tokens than V would go unnoticed, as
+        their words have room for up to 31 more, and forbid those tokens.)"""
+        if B != self.B:
+            raise ValueError("the rules are of another batch size")
+        if self.V not in (None, V):
+            raise ValueError(f"the masks are for {self.V} tokens, the logits have {V}")
+
     def release(self) -> None:
         if self._buf:
             self.s._lib.gorch_cuda_buffer_free(self._buf)
@@ -128,8 +141,7 @@ def adjust_logits(s: CudaSampler, logits, rules: LogitRules, in_place: bool = Fa
     from .sampling import _logits_arg
     a, dtype = _logits_arg(logits)
     B, V = a.shape
-    if B != rules.B:
-        raise ValueError("the rules are of another batch size")
+    rules.check(B, V)
     out = np.empty_like(a)
     bufs = _Bufs(s)
     try:
