@@ -169,8 +169,9 @@ def generate_on_device(model, prompts, cfgs, uniforms, sampler: CudaSampler, max
     `model.forward_dev(state)` each return (logits_ptr, dtype, V, row_stride) for logits [B,V]
     on the device. `rules` (rules.LogitRules of the B rows): penalties over each row's own tokens, biases and
     masks, applied to every step's logits where they lie (see DeviceGenerateState.step); `rules` may also be a
-    function of the step's number that returns them, for grammars whose masks change as tokens are added.
-    Returns DeviceGenerateState.results()."""
+    function of the step's number that returns them, for rules that are known before the tokens are. (The loop does not
+    wait for its tokens: a grammar whose masks follow what was sampled takes a loop of the caller's own over
+    DeviceGenerateState.step and results.) Returns DeviceGenerateState.results()."""
     cfgs = np.ascontiguousarray(cfgs, dtype=CFG_DTYPE)
     uniforms = np.ascontiguousarray(uniforms, dtype=np.float64).reshape(max(int(max_new), 0), -1)
     st = DeviceGenerateState(sampler, prompts, max_new, max_seq, stop_tokens, loop)
