@@ -99,20 +99,22 @@ struct LmHeadArgs {
 // on the x side, over the multiple of 32 batch rows that holds the run, with zeros in the rows around it. LMA_STAGE units share a
 // stage of the ring (32-byte rows, 32-byte swizzle; what a rank leaves of a unit is filled with zeros by the copy). Four warps of
 // their own ask for a stage's units, one each, once the producer has found the stage free and announced its bytes (256 rows with 32
-// adapters of rank 32 over 1,024 x 151,936: 225 us so, 355 with one thread asking for all, 401 with cp.async in place of TMA;
-// the projection alone 95). What bounds it: W and the b's are 121 us at the copy rate; a stage's way round the ring, with three
-// stages of 64 KB for 256 rows, is about 50 us of the rest, the MMAs 34, the loads 32 (six or eight units to a stage did not make it
-// faster: 276, 237). 64 rows with eight adapters of rank 16: 90 us (70 alone); one row: 70 (64).
+// adapters of rank 32 over 1,024 x 151,936: 225 us so, 355 with one thread asking for all, 401 with cp.async in place of TMA,
+// all with two parts of h and one sum (see below); now 235 to 245, and the projection alone 95). What bounds it: W and the b's are 121 us at
+// the copy rate; a stage's way round the ring, with three
+// stages of 64 KB for 256 rows, is about 50 us of the rest, the MMAs 34 (with two parts of h), the loads 32 (six or eight units to a stage did not make it
+// faster: 276, 237 for 225). 64 rows with eight adapters of rank 16: 93 us (70 alone); one row: 70 (53 alone).
 // So an adapter's b passes once per group, its products cost what its rows cost, rounded up to 32 (with every unit over all
-// rows of the item, 256 x 1,024 x 151,936 with 32 adapters of rank 32 took 290 us), and the epilogue's results are complete.
+// rows of the item, 256 x 1,024 x 151,936 with 32 adapters of rank 32 took 290 us, though 64 rows with eight of rank 16 took 83),
+// and the epilogue's results are complete.
 // h goes in as three bf16, eight bits of the f32 value after eight, each multiplied with the same tile of b: nothing of h is lost.
 // The tensor pipe cuts its sums off where f32 would round them, which over K = 1,024 puts 1.0e-6 of the logits' size on them, and in
 // proportion to K. So they are cut into runs of LMA_SEG products, each with an accumulator of its own (the last goes on over
 // the adapters), and the epilogue adds those in registers, rounding to nearest. Errors as a share of the logits' size, root mean squares
 // against 64 bits, 64 rows, rank 16: K = 1,024: 4.9e-7 (one sum: 1.0e-6; an f32 product: 2.5e-7), K = 4,096: 4.7e-7 (4.4e-6; 5.9e-7); rank 256:
 // 8.0e-7. Runs of 256 halve it and cost more: one row 70 -> 76 us, 256 rows with 32 adapters of rank 32 236 -> 277.
-// 0 times an Inf or NaN in an adapter's b is NaN, in the rows around its run too (and the parts of h may disagree about an Inf in the
-// row's own): where a group has adapters, the epilogue works a NaN out again from the row's own operands, unless x holds one.
+// 0 times an Inf or NaN in an adapter's b is NaN, in the rows around its run too (and so is a part of h that is 0 times an Inf of the row's
+// own): where a group has adapters, the epilogue's warps work the NaNs out again at their end, from the row's own operands, unless x holds one.
 constexpr int LMA_UNIT = 16;             // columns of the rank in a unit: K of one MMA, 32 bytes
 constexpr int LMA_PARTS = 3;             // bf16 that make up a value of h
 constexpr int LMA_SEG = 512;             // products of a sum on the tensor pipe
