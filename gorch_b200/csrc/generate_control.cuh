@@ -73,12 +73,20 @@ __device__ __noinline__ int gc_row_argmax(const GenControlArgs& A, int b, bu::Sc
   rv.init(static_cast<const T*>(A.logits) + b * A.row_stride, A.V);
   unsigned long long best = 0ull;
   bool odd = false;
-  for (int v = tid; v < rv.nvec; v += GC_NT) {
-    rv.visit(v, [&](float x, int i) {
-      odd |= !(x < INFINITY);
-      const unsigned long long p = (static_cast<unsigned long long>(okey(x)) << 32) | static_cast<uint32_t>(~i);
-      best = p > best ? p : best;
-    });
+  constexpr int U = 8;                                        // vectors of a thread on their way together
+  for (int v0 = tid; v0 < rv.nvec; v0 += U * GC_NT) {
+    uint4 raw[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) raw[u] = *(rv.vbase + min(v0 + u * GC_NT, rv.nvec - 1));
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      if (v0 + u * GC_NT >= rv.nvec) break;
+      rv.visit_raw(raw[u], v0 + u * GC_NT, [&](float x, int i, int) {
+        odd |= !(x < INFINITY);
+        const unsigned long long p = (static_cast<unsigned long long>(okey(x)) << 32) | static_cast<uint32_t>(~i);
+        best = p > best ? p : best;
+      });
+    }
   }
   best = bu::max_u64<GC_NT / 32>(best, sc, tid);
   if (__syncthreads_or(odd) || !(okey_to_float(static_cast<uint32_t>(best >> 32)) > -INFINITY)) return -1;
@@ -140,7 +148,7 @@ __global__ void __launch_bounds__(GC_NT) generate_control_kernel(const __grid_co
     // An id that the mask does not allow: it leaves nothing, or the row cannot be sampled from (NaN, +Inf), or the draw ran past the last
     // kept token, which gives V - 1 whatever the mask (rounding, with a uniform next to 1; mode A's top_p, which may
     // remove every token). In the last case the row's largest logit, which the mask allows, takes its place. All of them are rare, and end
-    // the row or happen once in a long while: a row's scan by this one CTA (10 us for 151,936 columns) is no cost to speak of.
+    // the row or happen once in a long while: a row's scan by this one CTA (30 us for 151,936 columns) is no cost to speak of.
     if (A.mask == nullptr || !__syncthreads_or(look)) continue;
     if (look) s_look[atomicAdd(&s_nlook, 1)] = b;
     __syncthreads();
